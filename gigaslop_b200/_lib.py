@@ -10,9 +10,10 @@ LIB_PATH = os.environ.get("GIGASLOP_B200_LIB") or os.path.join(_PKG, "libgigaslo
 OK = 0
 ERRORS = {-1: "bad argument", -2: "unsupported shape", -3: "device is not sm_100"}
 
-F16, F32 = 0, 1
+F16, F32, BF16 = 0, 1, 2
 FLAG_SCALAR_SCALE_B = 4
 FLAG_OWN_ROW_BLOCKS = 8
+FLAG_B_KN = 16
 
 _i32, _i64, _p = C.c_int32, C.c_int64, C.c_void_p
 
@@ -47,6 +48,14 @@ SIGNATURES = {
     "gsb200_mx_scales_to_tiled": (_i32, [_p, _i64, _i64, _i32, _p, _p]),
     "gsb200_gemm_mxfp8_f16": (_i32, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i32, _i32, _p]),
     "gsb200_dual_gemm_mxfp8_silu_f16": (_i32, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i32, _i32, _p]),
+    "gsb200_block_quantize_fp8": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p]),
+    "gsb200_block_dequantize_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i32, _i64, _i64, _i32, _i32, _p]),
+    "gsb200_gemm_fp8_block": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i32, _i32, _i32, _p]),
+    "gsb200_gemm_fp8_block_wgrad_workspace_bytes": (_i64, [_i64, _i32, _i32]),
+    "gsb200_gemm_fp8_block_wgrad": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _i64, _i32, _i32, _p]),
+    "gsb200_swiglu_fp8_block": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "gsb200_swiglu_fp8_block_bwd": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p,
+                                           _i64, _i64, _i64, _i32, _p]),
     "gsb200_lstm_scratch_bytes": (_i64, [_i64, _i32]),
     "gsb200_lstm_layer_fp8": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _p, _i64, _p]),
     "gsb200_lstm_layer_fp8_static": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _p]),

@@ -227,6 +227,46 @@ int32_t gsb200_dual_gemm_mxfp8_silu_f16(const uint8_t* A, int64_t lda, const uin
                         S(stream));
 }
 
+int32_t gsb200_block_quantize_fp8(const void* x, int32_t x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale,
+                                  int64_t M, int32_t K, int32_t block_rows, gsb200_stream_t stream) {
+  return launch_block_quantize(x, x_dtype, ldx, q, ldq, scale, ld_scale, M, K, block_rows, S(stream));
+}
+
+int32_t gsb200_block_dequantize_fp8(const uint8_t* q, int64_t ldq, const float* scale, int64_t ld_scale, void* x, int32_t x_dtype,
+                                    int64_t ldx, int64_t M, int32_t K, int32_t block_rows, gsb200_stream_t stream) {
+  return launch_block_dequantize(q, ldq, scale, ld_scale, x, x_dtype, ldx, M, K, block_rows, S(stream));
+}
+
+int32_t gsb200_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* scale_a, int64_t ld_scale_a, const uint8_t* B, int64_t ldb,
+                              const float* scale_b, int64_t ld_scale_b, void* C, int64_t ldc, int32_t c_dtype, int64_t M, int32_t N,
+                              int32_t K, int32_t flags, gsb200_stream_t stream) {
+  return launch_block_gemm(A, lda, scale_a, ld_scale_a, B, ldb, scale_b, ld_scale_b, C, ldc, c_dtype, M, N, K, flags, S(stream));
+}
+
+int64_t gsb200_gemm_fp8_block_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K) { return wgrad_workspace_bytes(M, N, K); }
+
+int32_t gsb200_gemm_fp8_block_wgrad(const void* dY, int32_t dy_dtype, int64_t lddy, const uint8_t* q, int64_t ldq, const float* scale,
+                                    int64_t ld_scale, float* dW, int64_t lddw, int32_t accumulate, void* workspace,
+                                    int64_t workspace_bytes, int64_t M, int32_t N, int32_t K, gsb200_stream_t stream) {
+  return launch_wgrad(dY, dy_dtype, lddy, q, ldq, scale, ld_scale, dW, lddw, accumulate, workspace, workspace_bytes, M, N, K, S(stream));
+}
+
+int32_t gsb200_swiglu_fp8_block(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int32_t dtype, uint8_t* h_q, float* h_s,
+                                uint8_t* gate_q, float* gate_s, uint8_t* up_q, float* up_s, int64_t ldq, int64_t ld_scale, int64_t M,
+                                int32_t F, gsb200_stream_t stream) {
+  return launch_swiglu_block(gate, ld_gate, up, ld_up, dtype, h_q, h_s, gate_q, gate_s, up_q, up_s, ldq, ld_scale, M, F, S(stream));
+}
+
+int32_t gsb200_swiglu_fp8_block_bwd(const void* dh, int32_t dtype, int64_t lddh, const uint8_t* gate_q, int64_t ld_gate_q,
+                                    const float* gate_s, int64_t ld_gate_s, const uint8_t* up_q, int64_t ld_up_q, const float* up_s,
+                                    int64_t ld_up_s, void* dgate, int64_t ld_dgate, void* dup, int64_t ld_dup, uint8_t* dgate_q,
+                                    float* dgate_s, uint8_t* dup_q, float* dup_s, int64_t ldq, int64_t ld_scale, int64_t M, int32_t F,
+                                    gsb200_stream_t stream) {
+  const SwigluBwd p{dh, lddh, gate_q, ld_gate_q, gate_s, ld_gate_s, up_q, ld_up_q, up_s, ld_up_s, dgate, ld_dgate, dup, ld_dup,
+                    {dgate_q, dup_q}, {dgate_s, dup_s}, ldq, ld_scale, M, F};
+  return launch_swiglu_block_bwd(p, dtype, S(stream));
+}
+
 int64_t gsb200_lstm_scratch_bytes(int64_t B, int32_t H) {
   if (B <= 0 || H <= 0) return 0;
   return static_cast<int64_t>(lstm_scratch_bytes(B, H));

@@ -78,6 +78,26 @@ int32_t launch_mx_scales_to_tiled(const uint8_t* src, long long ld, long long ro
 int32_t launch_mx_gemm(bool dual, const uint8_t* A, long long lda, const uint8_t* sfa, const uint8_t* B0,
                        const uint8_t* B1, long long ldb, const uint8_t* sfb0, const uint8_t* sfb1, void* C,
                        long long ldc, long long M, int N, int K, cudaStream_t st);
+int32_t launch_block_quantize(const void* x, int dt, long long ldx, uint8_t* q, long long ldq, float* scale, long long lds, long long M, int K,
+                              int block_rows, cudaStream_t st);
+int32_t launch_block_dequantize(const uint8_t* q, long long ldq, const float* scale, long long lds, void* x, int dt, long long ldx, long long M,
+                                int K, int block_rows, cudaStream_t st);
+int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb, const float* sb,
+                          long long ld_sb, void* C, long long ldc, int c_type, long long M, int N, int K, int flags, cudaStream_t st);
+int64_t wgrad_workspace_bytes(long long M, int N, int K);
+int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, long long ldq, const float* s, long long lds, float* dw, long long lddw,
+                     int accumulate, void* ws, long long ws_bytes, long long M, int N, int K, cudaStream_t st);
+int32_t launch_swiglu_block(const void* gate, long long ldg, const void* up, long long ldu, int dt, uint8_t* hq, float* hs, uint8_t* gq, float* gs,
+                            uint8_t* uq, float* us, long long ldq, long long lds, long long M, int F, cudaStream_t st);
+struct SwigluBwd {
+  const void* dh; long long lddh;
+  const uint8_t* gq; long long ldgq; const float* gs; long long ldgs;
+  const uint8_t* uq; long long lduq; const float* us; long long ldus;
+  void* dg; long long lddg; void* du; long long lddu;
+  uint8_t* q[2]; float* s[2]; long long ldq, lds;      // dgate and dup in the format as well, or null
+  long long M; int F;
+};
+int32_t launch_swiglu_block_bwd(const SwigluBwd& p, int dt, cudaStream_t st);
 int32_t launch_tensor_peak_probe(int kind, int n, int mmas, long long* clocks, int* ctas_out, cudaStream_t st);
 int32_t ensure_device();          // validates the current device once, returns GSB200_OK / error
 int sm_count();                   // SMs of the current device (cached), capped by set_sm_limit

@@ -6,5 +6,8 @@
 #include "lstm.cu"
 #include "factored.cu"
 #include "mx_gemm.cu"
+#include "block8.cu"
+#include "block_gemm.cu"
+#include "wgrad.cu"
 #include "probe.cu"
 #include "capi.cu"

@@ -286,6 +286,20 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for an operand whose rows are the reduction ("MN-major"): rows of 128 bytes along M or N with the 128-byte swizzle (a TMA
+// box of 128 bytes x rows), 8-row groups 1024 bytes apart (SBO), the next 128 bytes along M or N `lbo` bytes further (LBO).  Advancing
+// along K by r rows = adding r * 128 >> 4.  The instruction descriptor says which operand is one (UMMA_A_MN, UMMA_B_MN).
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t smem_addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(lbo >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+constexpr uint32_t UMMA_A_MN = 1u << 15, UMMA_B_MN = 1u << 16;
+
 // 16 bytes from registers into the shared memory of a CTA of the cluster, reported to an mbarrier of that CTA (both are
 // cluster addresses from mapa_shared).
 __device__ __forceinline__ void st_async_v4(uint32_t dst_cluster_addr, uint4 v, uint32_t mbar_cluster_addr) {
@@ -421,6 +435,12 @@ __device__ __forceinline__ void umma_f8_elect(uint32_t d_tmem, uint64_t a_desc, 
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // shared -> TMEM copy of scale factors (32 lanes x 128 bit, replicated to the 4 lane quarters)

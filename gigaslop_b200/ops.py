@@ -488,3 +488,205 @@ def _checked_dual_gemm_mxfp8_silu(A, sfa_tiled, B_gate, B_up, sfb_gate_tiled, sf
                                                 sfb_up_tiled.data_ptr(), C.data_ptr(), C.stride(0), M, N, K, _stream()),
           "dual_gemm_mxfp8_silu")
     return C
+
+
+# ---- block-scaled FP8: one fp32 scale per 128 elements of a row, or per 128 x 128 tile ---------------------------------
+BLOCK = 128
+_BLOCK_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def _block_dt(t, name, allowed=(torch.float16, torch.bfloat16, torch.float32)):
+    dt = t if isinstance(t, torch.dtype) else t.dtype
+    if dt not in allowed:
+        raise TypeError(f"{name} must be one of {tuple(allowed)}, not {dt}")
+    return _BLOCK_DT[dt]
+
+
+def _blocks(n):
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _rows16(m, n, dtype, device):
+    """An [m, n] output whose rows start on 16-byte boundaries: what the tensor cores read, and the fast stores."""
+    per = 16 // dtype.itemsize
+    ld = (n + per - 1) // per * per
+    t = torch.empty((m, ld), dtype=dtype, device=device)
+    return t if ld == n else t[:, :n]
+
+
+def _given(t, shape, dtypes, name):
+    """A tensor argument of this shape and one of these types, rows of unit stride that do not overlap."""
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    if shape[0] == 0 or shape[1] == 0:
+        return t
+    if (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
+        raise ValueError(f"{name} must have unit inner stride and rows that do not overlap")
+    return t
+
+
+def _ld(t):
+    """Row stride for the library; of a single row it says nothing, so the least that is aligned for any use."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def _f8_scaled(q, s, rows, name):
+    if q.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    _given(q, q.shape, _F8, name)
+    _given(s, (_blocks(q.shape[0]) if rows == BLOCK else q.shape[0], _blocks(q.shape[1])), (torch.float32,), f"scale of {name}")
+
+
+def _2d(t, name):
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    return _given(t, t.shape, (t.dtype,), name)
+
+
+def fp8_block_quantize(x, rows=1, out=None, out_scale=None):
+    """``x`` [M,K] fp16/bf16/fp32 -> (float8_e4m3fn [M,K], fp32 scales): one scale per 128 elements of a row (``rows=1``, activations,
+    gradients and checkpoints: scales [M, ceil(K/128)]) or per 128 x 128 tile (``rows=128``, weights: [ceil(M/128), ceil(K/128)]).
+    Scales are the smallest powers of two with ``max|x| <= 448 * scale``.  The elements' rows start on 16-byte boundaries, as the
+    products want them."""
+    return _checked_fp8_block_quantize(x, rows, out, out_scale)
+
+
+@_on_device
+def _checked_fp8_block_quantize(x, rows, out, out_scale):
+    _need_cuda(x)
+    _2d(x, "x")
+    dt = _block_dt(x, "x")
+    if rows not in (1, BLOCK):
+        raise ValueError("a block is 1 or 128 rows")
+    M, K = x.shape
+    sshape = (_blocks(M) if rows == BLOCK else M, _blocks(K))
+    q = _given(out, (M, K), _F8, "out") if out is not None else _rows16(M, K, torch.float8_e4m3fn, x.device)
+    s = _given(out_scale, sshape, (torch.float32,), "out_scale") if out_scale is not None else torch.empty(sshape, dtype=torch.float32, device=x.device)
+    check(lib().gsb200_block_quantize_fp8(x.data_ptr(), dt, _ld(x), q.data_ptr(), _ld(q), s.data_ptr(), max(_ld(s), sshape[1]), M, K, rows, _stream()),
+          "fp8_block_quantize")
+    return q, s
+
+
+def fp8_block_dequantize(q, scale, rows=1, dtype=torch.bfloat16, out=None):
+    """The values ``q * scale`` of a block-scaled tensor as fp16, bf16 or fp32 (a checkpoint restored, for a backward pass of the
+    caller's own).  Exact in bf16 and fp32 for scales that are powers of two."""
+    return _checked_fp8_block_dequantize(q, scale, rows, dtype, out)
+
+
+@_on_device
+def _checked_fp8_block_dequantize(q, scale, rows, dtype, out):
+    _need_cuda(q, scale)
+    if rows not in (1, BLOCK):
+        raise ValueError("a block is 1 or 128 rows")
+    _f8_scaled(q, scale, rows, "q")
+    M, K = q.shape
+    if out is not None:
+        _2d(out, "out")
+        dtype = out.dtype
+    dt = _block_dt(dtype, "out")
+    x = _given(out, (M, K), (dtype,), "out") if out is not None else _rows16(M, K, dtype, q.device)
+    check(lib().gsb200_block_dequantize_fp8(q.data_ptr(), _ld(q), scale.data_ptr(), _ld(scale), x.data_ptr(), dt, _ld(x), M, K, rows, _stream()),
+          "fp8_block_dequantize")
+    return x
+
+
+def gemm_fp8_block(A, B, scale_a, scale_b, out=None, dtype=torch.float16, b_transposed=False):
+    """``A[M,K] . B[N,K]^T`` over block-scaled FP8 operands -> fp16, bf16 or fp32: ``scale_a`` [M, ceil(K/128)], ``scale_b``
+    [ceil(N/128), ceil(K/128)].  ``b_transposed``: B is [K,N] with scales [ceil(K/128), ceil(N/128)], which is the input gradient
+    ``dY . W`` with the weight as the forward pass has it.  Sums and scales in fp32, one rounding."""
+    return _checked_gemm_fp8_block(A, B, scale_a, scale_b, out, dtype, b_transposed)
+
+
+@_on_device
+def _checked_gemm_fp8_block(A, B, scale_a, scale_b, out, dtype, b_transposed):
+    _need_cuda(A, B, scale_a, scale_b)
+    _f8_scaled(A, scale_a, 1, "A")
+    _f8_scaled(B, scale_b, BLOCK, "B")
+    M, K = A.shape
+    Kb, N = B.shape if b_transposed else B.shape[::-1]
+    if Kb != K:
+        raise ValueError(f"A is [M,K] with K = {K}, B {'[K,N]' if b_transposed else '[N,K]'} with K = {Kb}")
+    if out is not None:
+        _2d(out, "out")
+        dtype = out.dtype
+    dt = _block_dt(dtype, "out")
+    C = _given(out, (M, N), (dtype,), "out") if out is not None else _rows16(M, N, dtype, A.device)
+    check(lib().gsb200_gemm_fp8_block(A.data_ptr(), _ld(A), scale_a.data_ptr(), _ld(scale_a), B.data_ptr(), _ld(B), scale_b.data_ptr(),
+                                      _ld(scale_b), C.data_ptr(), _ld(C), dt, M, N, K, _lib.FLAG_B_KN if b_transposed else 0, _stream()),
+          "gemm_fp8_block")
+    return C
+
+
+def gemm_fp8_block_wgrad(dy, q, scale, out=None, accumulate=False):
+    """Weight gradient ``dY^T . X`` [N,K] fp32 from ``dy`` [M,N] fp16/bf16 and the block-scaled 8-bit checkpoint ``q`` [M,K],
+    ``scale`` [M, ceil(K/128)] of the layer's input.  ``accumulate`` adds to ``out``.  Rows of ``dy`` on 16-byte boundaries."""
+    return _checked_gemm_fp8_block_wgrad(dy, q, scale, out, accumulate)
+
+
+@_on_device
+def _checked_gemm_fp8_block_wgrad(dy, q, scale, out, accumulate):
+    _need_cuda(dy, q, scale)
+    _2d(dy, "dy")
+    dt = _block_dt(dy, "dy", (torch.float16, torch.bfloat16))
+    _f8_scaled(q, scale, 1, "q")
+    (M, N), K = dy.shape, q.shape[1]
+    if q.shape[0] != M:
+        raise ValueError(f"dy has {M} rows, the checkpoint {q.shape[0]}")
+    if accumulate and out is None:
+        raise ValueError("accumulate needs the tensor to add to as out")
+    dw = _given(out, (N, K), (torch.float32,), "out") if out is not None else torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    need = int(lib().gsb200_gemm_fp8_block_wgrad_workspace_bytes(M, N, K))
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    check(lib().gsb200_gemm_fp8_block_wgrad(dy.data_ptr(), dt, _ld(dy), q.data_ptr(), _ld(q), scale.data_ptr(), _ld(scale), dw.data_ptr(), _ld(dw),
+                                            1 if accumulate else 0, ws.data_ptr() if need else None, need, M, N, K, _stream()),
+          "gemm_fp8_block_wgrad")
+    return dw
+
+
+def swiglu_fp8_block(gate, up):
+    """``gate * sigmoid(gate) * up`` as a block-scaled FP8 tensor, with 8-bit checkpoints of both inputs: ``((h, scale), (gate, scale),
+    (up, scale))``, each what ``fp8_block_quantize`` makes (of ``h``: from its fp32 values)."""
+    return _checked_swiglu_fp8_block(gate, up)
+
+
+@_on_device
+def _checked_swiglu_fp8_block(gate, up):
+    _need_cuda(gate, up)
+    _2d(gate, "gate")
+    dt = _block_dt(gate, "gate")
+    _given(up, gate.shape, (gate.dtype,), "up")
+    M, F = gate.shape
+    q = [_rows16(M, F, torch.float8_e4m3fn, gate.device) for _ in range(3)]
+    s = [torch.empty((M, _blocks(F)), dtype=torch.float32, device=gate.device) for _ in range(3)]
+    check(lib().gsb200_swiglu_fp8_block(gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up), dt, q[0].data_ptr(), s[0].data_ptr(), q[1].data_ptr(),
+                                        s[1].data_ptr(), q[2].data_ptr(), s[2].data_ptr(), q[0].stride(0), s[0].stride(0), M, F, _stream()),
+          "swiglu_fp8_block")
+    return (q[0], s[0]), (q[1], s[1]), (q[2], s[2])
+
+
+def swiglu_fp8_block_bwd(dh, gate_q, gate_scale, up_q, up_scale, quantize=False):
+    """Gradients of SwiGLU from the checkpoints: ``(dgate, dup)`` in ``dh``'s type.  ``quantize``: also ``(q, scale)`` of each, as
+    ``fp8_block_quantize`` makes of them, in the same pass: ``(dgate, dup, (q, scale), (q, scale))``."""
+    return _checked_swiglu_fp8_block_bwd(dh, gate_q, gate_scale, up_q, up_scale, quantize)
+
+
+@_on_device
+def _checked_swiglu_fp8_block_bwd(dh, gate_q, gate_scale, up_q, up_scale, quantize):
+    _need_cuda(dh, gate_q, gate_scale, up_q, up_scale)
+    _2d(dh, "dh")
+    dt = _block_dt(dh, "dh")
+    _f8_scaled(gate_q, gate_scale, 1, "gate_q")
+    _f8_scaled(up_q, up_scale, 1, "up_q")
+    M, F = dh.shape
+    if tuple(gate_q.shape) != (M, F) or tuple(up_q.shape) != (M, F):
+        raise ValueError(f"dh is {[M, F]}, the checkpoints {list(gate_q.shape)} and {list(up_q.shape)}")
+    dg, du = (_rows16(M, F, dh.dtype, dh.device) for _ in range(2))
+    q = [_rows16(M, F, torch.float8_e4m3fn, dh.device) for _ in range(2 if quantize else 0)]
+    s = [torch.empty((M, _blocks(F)), dtype=torch.float32, device=dh.device) for _ in q]
+    extra = (q[0].data_ptr(), s[0].data_ptr(), q[1].data_ptr(), s[1].data_ptr(), q[0].stride(0), s[0].stride(0)) if quantize else (None, None, None, None, 0, 0)
+    check(lib().gsb200_swiglu_fp8_block_bwd(dh.data_ptr(), dt, _ld(dh), gate_q.data_ptr(), _ld(gate_q), gate_scale.data_ptr(), _ld(gate_scale),
+                                            up_q.data_ptr(), _ld(up_q), up_scale.data_ptr(), _ld(up_scale), dg.data_ptr(), dg.stride(0),
+                                            du.data_ptr(), du.stride(0), *extra, M, F, _stream()), "swiglu_fp8_block_bwd")
+    return (dg, du, (q[0], s[0]), (q[1], s[1])) if quantize else (dg, du)

@@ -34,12 +34,14 @@ extern "C" {
 
 #define GSB200_F16 0
 #define GSB200_F32 1
+#define GSB200_BF16 2                /* the block-scaled FP8 entry points only */
 
 /* bit flags for the `flags` argument of the GEMM entry points; any other bit is rejected with GSB200_ERR_BAD_ARG */
 #define GSB200_FLAG_SCALAR_SCALE_B 4  /* plain dequant GEMMs: scale_b points to ONE fp32 used for every output column */
 /* Rotary GEMMs share the row blocks of the last, incomplete round among the CTAs that would idle (3.7 % faster alone
  * at M = 65536).  A caller that fills those SMs itself, with another kernel on a second stream, switches that off. */
 #define GSB200_FLAG_OWN_ROW_BLOCKS 8
+#define GSB200_FLAG_B_KN 16           /* gsb200_gemm_fp8_block: B is [K,N], its rows are the reduction */
 
 typedef struct CUstream_st* gsb200_stream_t; /* == cudaStream_t */
 
@@ -236,6 +238,58 @@ int32_t gsb200_dual_gemm_mxfp8_silu_f16(const uint8_t* A, int64_t lda, const uin
                                         const uint8_t* B_up, int64_t ldb, const uint8_t* sfb_gate_tiled,
                                         const uint8_t* sfb_up_tiled, void* C, int64_t ldc, int64_t M, int32_t N,
                                         int32_t K, gsb200_stream_t stream);
+
+/* Block-scaled FP8: E4M3 elements with one fp32 scale per 128 consecutive elements of a row (activations, gradients,
+ * checkpoints: scale [M, ceil(K/128)]) or per 128 x 128 tile (weights: scale [ceil(N/128), ceil(K/128)]); the value of an element is
+ * q * scale, and the last block of a row may be shorter.  The same quantised activations are the forward product's operand and the
+ * 8-bit checkpoint that the backward pass reads.  No reference counterpart.
+ * Types: GSB200_F16, GSB200_BF16 and GSB200_F32 where nothing else is said.  Sizes: M arbitrary (0 does nothing), K, N and F arbitrary
+ * up to 2^30.  Row strides are in elements and may be any that hold a row, except for the operands that the tensor cores read (E4M3
+ * of the products: base 16-byte aligned, stride a multiple of 16; dY: base 16-byte aligned, stride a multiple of 8); rows on 16-byte
+ * boundaries are the fast ones elsewhere.  Nothing behind a row's last element is written.  Outputs must not overlap inputs.
+ *
+ * gsb200_block_quantize_fp8: scale = the smallest power of two s >= 2^-126 with max|x| <= 448 s over the block's finite elements (1 where
+ * they are all zero), q = e4m3(x / s) rounded to nearest even; NaN and infinities become NaN.  block_rows: 1 (a scale per row and
+ * block) or 128 (per tile).  A power of two loses nothing in a floating-point element type and makes the division exact.
+ * gsb200_block_dequantize_fp8: x = q * scale rounded to x's type; any scales. */
+int32_t gsb200_block_quantize_fp8(const void* x, int32_t x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale,
+                                  int64_t M, int32_t K, int32_t block_rows, gsb200_stream_t stream);
+int32_t gsb200_block_dequantize_fp8(const uint8_t* q, int64_t ldq, const float* scale, int64_t ld_scale, void* x, int32_t x_dtype,
+                                    int64_t ldx, int64_t M, int32_t K, int32_t block_rows, gsb200_stream_t stream);
+
+/* C[m,n] = sum over blocks b of scale_a[m,b] * scale_b[n/128,b] * (sum over k in b of A[m,k] B[n,k]): fp32 sums, one rounding to C's type.
+ * A [M,K] with scales per row and block, B [N,K] with scales per tile; any fp32 scales whose products are finite.  One row to many.
+ * flags = GSB200_FLAG_B_KN: B is [K,N] with scale_b[k/128, n/128].  That is the input gradient dX = dY . W with W and its scales as the
+ * forward pass has them (A = the quantised dY, K = the layer's outputs, N = its inputs).  C: any alignment (16-byte rows are the
+ * fast ones). */
+int32_t gsb200_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* scale_a, int64_t ld_scale_a, const uint8_t* B, int64_t ldb,
+                              const float* scale_b, int64_t ld_scale_b, void* C, int64_t ldc, int32_t c_dtype, int64_t M, int32_t N,
+                              int32_t K, int32_t flags, gsb200_stream_t stream);
+
+/* Weight gradient from an 8-bit checkpoint: dW[n,k] = sum over m of dY[m,n] * (scale[m,k/128] q[m,k]), fp32 sums and fp32 dW;
+ * accumulate != 0 adds to what dW holds (gradient accumulation).  dY fp16 or bf16 [M,N], q / scale as the forward pass's quantiser left
+ * them [M,K].  q * scale is rounded to dY's type on its way to the tensor cores: exact for scales that are powers of two (fp16: and values
+ * up to 65504).  The order of the sums depends on the sizes alone.  M = 0 gives zeros (or leaves dW as it is).
+ * workspace: gsb200_gemm_fp8_block_wgrad_workspace_bytes(M, N, K) bytes (may be 0), 32-byte aligned; calls that may overlap
+ * need one each. */
+int64_t gsb200_gemm_fp8_block_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K);
+int32_t gsb200_gemm_fp8_block_wgrad(const void* dY, int32_t dy_dtype, int64_t lddy, const uint8_t* q, int64_t ldq, const float* scale,
+                                    int64_t ld_scale, float* dW, int64_t lddw, int32_t accumulate, void* workspace,
+                                    int64_t workspace_bytes, int64_t M, int32_t N, int32_t K, gsb200_stream_t stream);
+
+/* SwiGLU into the format, with checkpoints: h = gate * sigmoid(gate) * up in fp32, quantised from there (the down-projection's operand), and
+ * gate and up quantised for the backward pass.  gate, up [M,F] of one type; the three outputs share their row strides.
+ * The gradient reads the checkpoints (any scales): with s = sigmoid(gate), dup = dh * gate * s, dgate = dh * up * s * (1 + gate * (1 - s)), in
+ * dh's type.  dgate_q .. dup_s (all four or none): the two gradients quantised as well, from their rounded values, for the input gradient's
+ * product. */
+int32_t gsb200_swiglu_fp8_block(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int32_t dtype, uint8_t* h_q, float* h_s,
+                                uint8_t* gate_q, float* gate_s, uint8_t* up_q, float* up_s, int64_t ldq, int64_t ld_scale, int64_t M,
+                                int32_t F, gsb200_stream_t stream);
+int32_t gsb200_swiglu_fp8_block_bwd(const void* dh, int32_t dtype, int64_t lddh, const uint8_t* gate_q, int64_t ld_gate_q,
+                                    const float* gate_s, int64_t ld_gate_s, const uint8_t* up_q, int64_t ld_up_q, const float* up_s,
+                                    int64_t ld_up_s, void* dgate, int64_t ld_dgate, void* dup, int64_t ld_dup, uint8_t* dgate_q,
+                                    float* dgate_s, uint8_t* dup_q, float* dup_s, int64_t ldq, int64_t ld_scale, int64_t M, int32_t F,
+                                    gsb200_stream_t stream);
 
 /* LSTM layer, recurrent half: T sequential steps in one persistent kernel (thread-block clusters exchanging h through
  * distributed shared memory for H <= 384; a cooperative kernel with global scratch otherwise).
