@@ -8,10 +8,18 @@
 // The scales change along the reduction, so the tensor core cannot carry a sum over a whole row: each 128-wide K block is multiplied into a
 // tensor-memory stage of its own (four MMAs of K = 32 that start from zero), and the epilogue warps add it, times its scale, to fp32 sums
 // in registers: one fused multiply-add per element and K block, since a thread holds one row and 128 columns that share a B scale.
-// Tile 128 rows x 256 columns: per K block 512 tensor clocks, and for the eight epilogue warps 256 clocks of multiply-adds and as many
-// of tensor-memory reads.  Two stages of 256 TMEM columns let both sides run at once.
-//   warp 0      TMA producer (one lane)       warp 1   MMA issue (converged, one elected lane)
+//
+// Large form: CTA pairs (cta_group::2), tile 256 rows x 256 columns, 128 x 256 per CTA, two tensor-memory stages of 256 columns.
+//   warp 0      TMA producer (one lane); a CTA loads its 128 rows of A and half of the tile's B, 32 KiB per K block
+//   warp 1      MMA issue (first CTA of the pair; converged, one elected lane)
+//   warps 2, 3  products of the scales, two K blocks ahead, through shared memory
 //   warps 4..11 epilogue: lane quarter e % 4, column half e / 4
+// What bounds it is the round trip of a stage, two of which are all that tensor memory holds: MMAs (512 clocks and about 230 until the last
+// one shows), the epilogue's wake-up, four reads of 32 columns (300), the return to the MMA warp (230): about 1700 clocks for two
+// K blocks, 850 each where the MMAs alone take 512.  Everything that can leave that chain has left it: the scales (their address arithmetic,
+// loads and products), the wait for the operands (before that for the stage), the multiply-adds of a chunk (behind the read of the next one,
+// the last ones behind the release).  us, M = 65536, N = 1536, K = 512 / N = 512, K = 2048: single CTAs with 256 columns that load their own scales
+// 91 / 80; pairs 95 / 80; scales through shared memory 78 / 76; two staging boxes per warp instead of one 72 / 74.
 #include <atomic>
 
 #include "capi_internal.h"
@@ -19,24 +27,32 @@
 
 namespace gsb {
 
-constexpr int BG_BM = 128, BG_BK = 128;
+constexpr int BG_BM = 128, BG_BN = 256, BG_BK = 128;
 constexpr int BG_EPI_WARPS = 8, BG_FRONT_WARPS = 4;
+constexpr int BG_FRONT_REGS = 56, BG_EPI_REGS = 224;
 constexpr int BG_THREADS = 32 * (BG_EPI_WARPS + BG_FRONT_WARPS);
 constexpr int BG_A_BYTES = BG_BM * BG_BK;                  // 16 KiB
-constexpr int BG_STAGES = 4;
-constexpr int BG_OUT_BUF = 4096;                           // per epilogue warp: 32 rows of 128 bytes
+constexpr int BG_ACC = 2;                                  // tensor-memory stages
+constexpr int BG_OUT_BUF = 2 * 4096;                       // per epilogue warp: two boxes of 32 rows x 128 bytes
 
-template <int BN>
-struct BgSmem {
-  static constexpr int STAGE = BG_A_BYTES + BN * BG_BK;
-  static constexpr int OUT = BG_STAGES * STAGE;
-  static constexpr int BAR = OUT + BG_EPI_WARPS * BG_OUT_BUF;
-  static constexpr int BYTES = BAR + 256 + 1024;
-  static_assert(BYTES <= 227 * 1024, "shared memory budget");
-};
+constexpr int BG_SC = 4;                                   // K blocks of scales in shared memory
+
+constexpr int BG_B_BYTES = BG_BN / 2 * BG_BK;              // a CTA of the pair holds half of the tile's columns
+constexpr int BG_STAGE = BG_A_BYTES + BG_B_BYTES;          // 32 KiB
+constexpr int BG_STAGES = 4;
+constexpr int BG_OUT = BG_STAGES * BG_STAGE;
+constexpr int BG_SCALES = BG_OUT + BG_EPI_WARPS * BG_OUT_BUF;             // [BG_SC][2][BG_BM] products of the scales
+constexpr int BG_BAR = BG_SCALES + BG_SC * 2 * BG_BM * 4;
+constexpr int BG_BYTES = BG_BAR + 256 + 1024;
+static_assert(BG_BYTES <= 227 * 1024, "shared memory budget");
+
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 struct BgParams {
-  int M, N, m_blocks, n_blocks, k_blocks;
+  int M, N, m_blocks, n_blocks, k_blocks;                  // a pair's row block is 256 rows, 128 per CTA
   const float* sa; long long ld_sa;
   const float* sb; long long ld_sb_n, ld_sb_k;             // B scale of (column block, K block): sb[cb * ld_sb_n + kb * ld_sb_k]
   void* C; long long ldc; int c_type;
@@ -44,129 +60,181 @@ struct BgParams {
 };
 
 // KN: B is [K, N].  Its stage holds boxes of 128 K rows x 128 columns.
-template <int BN, bool KN>
+template <bool KN>
 __global__ void __launch_bounds__(BG_THREADS, 1)
 block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_c,
                   const BgParams p) {
   extern __shared__ uint8_t bg_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(bg_smem_raw) + 1023) & ~uintptr_t(1023));
-  using L = BgSmem<BN>;
-  constexpr int ACC = 512 / BN > 4 ? 4 : 512 / BN;         // accumulator stages
+  constexpr int BN = BG_BN, ACC = BG_ACC, STAGES = BG_STAGES;
   constexpr int CW = BN / 2;                               // columns of an epilogue warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* empty = full + BG_STAGES;
-  uint64_t* acc_full = empty + BG_STAGES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + BG_BAR);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + ACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACC);
+  float* sc_smem = reinterpret_cast<float*>(smem + BG_SCALES);
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_tiles = p.m_blocks * p.n_blocks;           // (the host keeps this below 2^31)
+  const int rank = (int)cluster_ctarank();      // the pair's first CTA issues the MMAs; its barriers collect both CTAs' loads and releases
+  const int unit = (int)(blockIdx.x >> 1), units = (int)(gridDim.x >> 1);
+  auto tile_row = [&](int t) { return t / p.n_blocks * 2 * BG_BM + rank * BG_BM; };      // this CTA's first row
+  auto tile_col = [&](int t) { return t % p.n_blocks * BN; };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < BG_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int s = 0; s < ACC; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], BG_EPI_WARPS); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < ACC; ++s) { mbar_init(&acc_full[s], 1 + 2); mbar_init(&acc_empty[s], 2 * BG_EPI_WARPS); }
     abort_flag.set(0);
     fence_mbar_init();
     prefetch_tmap(&tm_a); prefetch_tmap(&tm_b); prefetch_tmap(&tm_c);
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, ACC * BN); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc_pair(tmem_slot, ACC * BN); tmem_relinquish_pair(); }
   pdl_wait();
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();                                      // (a __syncthreads of both CTAs) the other's barriers are initialised before anything arrives at them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const unsigned int budget = spin_budget();
 
   if (warp < BG_FRONT_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BG_FRONT_REGS));
     if (warp == 0) {
       if (lane == 0) {
         bool ok = true;
         int s = 0; uint32_t ph = 0;
-        for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
-          const int m0 = t / p.n_blocks * BG_BM, n0 = t % p.n_blocks * BN;
+        for (int t = unit; ok && t < num_tiles; t += units) {
+          const int m0 = tile_row(t), n0 = tile_col(t) + rank * (BN / 2);
           for (int kb = 0; kb < p.k_blocks; ++kb) {
             if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE00 | s, budget)) { ok = false; break; }
-            uint8_t* st = smem + s * L::STAGE;
-            mbar_arrive_expect_tx(&full[s], L::STAGE);
-            tma_load_2d(st, &tm_a, &full[s], kb * BG_BK, m0);
-            if constexpr (KN) {
-#pragma unroll
-              for (int j = 0; j < (BN + 127) / 128; ++j) tma_load_2d(st + BG_A_BYTES + j * 128 * BG_BK, &tm_b, &full[s], n0 + 128 * j, kb * BG_BK);
-            } else {
-              tma_load_2d(st + BG_A_BYTES, &tm_b, &full[s], kb * BG_BK, n0);
-            }
-            if (++s == BG_STAGES) { s = 0; ph ^= 1; }
+            uint8_t* st = smem + s * BG_STAGE;
+            auto load = [&](void* dst, const CUtensorMap* m, int x, int y) {
+              tma_load_2d_pair(dst, m, mapa_shared(smem_u32(&full[s]), 0), x, y);
+            };
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * BG_STAGE);
+            load(st, &tm_a, kb * BG_BK, m0);
+            if constexpr (KN) load(st + BG_A_BYTES, &tm_b, n0, kb * BG_BK);
+            else load(st + BG_A_BYTES, &tm_b, kb * BG_BK, n0);
+            if (++s == STAGES) { s = 0; ph ^= 1; }
           }
         }
         if (!ok) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }     // loads in flight land before the CTA exits
       }
-    } else if (warp == 1) {
-      constexpr uint32_t idesc = umma_idesc(1, 0, 0, BG_BM, BN) | (KN ? UMMA_B_MN : 0u);
+    } else if (warp == 1 && rank == 0) {
+      constexpr uint32_t idesc = umma_idesc(1, 0, 0, 2 * BG_BM, BN) | (KN ? UMMA_B_MN : 0u);
       bool ok = true;
       int s = 0, as = 0; uint32_t ph = 0, aph = 0;
-      for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
+      for (int t = unit; ok && t < num_tiles; t += units) {
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE10 | as, budget)) ||
-              !__all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xE20 | s, budget))) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * L::STAGE);
+          // (the stage's return last: it is what the MMAs wait for)
+          if (!__all_sync(0xffffffffu, mbar_wait<true>(&full[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xE20 | s, budget))) { ok = false; break; }
+          const uint32_t st = smem_u32(smem + s * BG_STAGE);
           const uint64_t a_desc = umma_smem_desc_sw128(st);
-          const uint64_t b_desc = KN ? umma_smem_desc_mn(st + BG_A_BYTES, 128 * BG_BK) : umma_smem_desc_sw128(st + BG_A_BYTES);
+          const uint64_t b_desc = KN ? umma_smem_desc_mn<128>(st + BG_A_BYTES, 128 * BG_BK) : umma_smem_desc_sw128(st + BG_A_BYTES);
+          if (!__all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE10 | as, budget))) { ok = false; break; }
+          tc_fence_after();
           constexpr uint64_t b_step = KN ? (32 * 128) >> 4 : 2;           // K = 32: 32 rows of 128 bytes, or 32 bytes of a row
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f8_elect(tmem_base + as * BN, a_desc + 2 * k, b_desc + b_step * k, idesc, k != 0);
-          umma_commit_elect(&empty[s]);
-          umma_commit_elect(&acc_full[as]);
-          if (++s == BG_STAGES) { s = 0; ph ^= 1; }
+          for (int k = 0; k < 4; ++k) umma_f8_pair_elect(tmem_base + as * BN, a_desc + 2 * k, b_desc + b_step * k, idesc, k != 0);
+          umma_commit_pair_both_elect(&acc_full[as]);
+          umma_commit_pair_both_elect(&empty[s]);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
           if (++as == ACC) { as = 0; aph ^= 1; }
         }
       }
+    } else if (warp >= 2) {
+      // The products of the scales, ahead of the MMAs: two rows and both column halves per lane, loaded two K blocks ahead.  A K
+      // block's arrival completes acc_full together with the MMAs' (the one wait of the epilogue covers both), and must follow the
+      // barrier's previous phase.  By then the MMAs two K blocks back were allowed to start, so the epilogue is done with the K block four
+      // back, whose place this one takes.
+      const int r = (warp - 2) * 64 + lane;
+      float a0[2], a1[2], b0[2], b1[2];
+      int ft = unit, fkb = 0;                                // what is fetched next
+      auto fetch_next = [&](int j) {
+        if (ft < num_tiles) {
+          const int m = tile_row(ft) + r, n = tile_col(ft);
+          a0[j] = ldg_f_here(p.sa + (long long)(m < p.M ? m : p.M - 1) * p.ld_sa + fkb);
+          a1[j] = ldg_f_here(p.sa + (long long)(m + 32 < p.M ? m + 32 : p.M - 1) * p.ld_sa + fkb);
+          const float* sb = p.sb + (long long)fkb * p.ld_sb_k + (long long)(n >> 7) * p.ld_sb_n;
+          b0[j] = ldg_f_here(sb);
+          b1[j] = n + 128 < p.N ? ldg_f_here(sb + p.ld_sb_n) : 0.f;
+        }
+        if (++fkb == p.k_blocks) { fkb = 0; ft += units; }
+      };
+      a0[0] = a0[1] = a1[0] = a1[1] = b0[0] = b0[1] = b1[0] = b1[1] = 0.f;
+      fetch_next(0);
+      fetch_next(1);
+      bool ok = true;
+      uint32_t i = 0;
+      auto put = [&](int j) {
+        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait<true>(&acc_full[j], ((i - 2) >> 1) & 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE40 | j, budget))) { ok = false; return; }
+        float* d = sc_smem + (i & (BG_SC - 1)) * 2 * BG_BM + r;
+        d[0] = a0[j] * b0[j]; d[32] = a1[j] * b0[j]; d[BG_BM] = a0[j] * b1[j]; d[BG_BM + 32] = a1[j] * b1[j];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_full[j]);
+        fetch_next(j);
+        ++i;
+      };
+      for (int t = unit; ok && t < num_tiles; t += units)
+        for (int kb = 0; ok && kb < p.k_blocks; ++kb) { if (i & 1) put(1); else put(0); }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BG_EPI_REGS));
     const int e = warp - BG_FRONT_WARPS, q = warp & 3, half = e >> 2;
-    uint8_t* const out_buf = smem + L::OUT + e * BG_OUT_BUF;
     const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + half * CW;
     bool ok = true;
-    int as = 0; uint32_t aph = 0;
-    for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
-      const int m0 = t / p.n_blocks * BG_BM + q * 32, n0 = t % p.n_blocks * BN + half * CW;
+    const float* const sc_lane = sc_smem + half * BG_BM + q * 32 + lane;
+    const uint32_t release_addr = mapa_shared(smem_u32(&acc_empty[0]), 0);
+    uint32_t it = 0;                                         // K blocks so far: stage it % 2, phase it / 2 % 2
+    static_assert(ACC == 2, "");
+    for (int t = unit; ok && t < num_tiles; t += units) {
+      const int m0 = tile_row(t) + q * 32, n0 = tile_col(t) + half * CW;
       const int row = m0 + lane;
       const bool live = m0 < p.M && n0 < p.N;                // (uniform) this warp has something to write
-      const float* sa = p.sa + (long long)(row < p.M ? row : p.M - 1) * p.ld_sa;
-      const float* sb = p.sb + (long long)((n0 < p.N ? n0 : 0) >> 7) * p.ld_sb_n;
       float acc[CW];
 #pragma unroll
       for (int i = 0; i < CW; ++i) acc[i] = 0.f;
-      float na = sa[0], nb = sb[0];                          // the next K block's scales
+      // A chain of 32-column chunks: while one is added, the next is on its way from tensor memory, across K blocks too if the next
+      // stage is there already; a stage goes back as soon as its last chunk is in registers.
+      uint32_t v[2][32];
+      auto stage_there = [&]() { return __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[it & 1], (it >> 1) & 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xE30, budget)); };
+      ok = stage_there();
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        const float sc = na * nb;
-        if (kb + 1 < p.k_blocks) { na = sa[kb + 1]; nb = sb[(long long)(kb + 1) * p.ld_sb_k]; }
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[as], aph, abort_flag, ST_TIMEOUT_EPILOGUE, 0xE30 | as, budget))) { ok = false; break; }
-        tc_fence_after();
-        if (live) {
-          const uint32_t ta = t_lane + as * BN;
-          const float2 s2 = pk2(sc, sc);
-          constexpr int NC = CW / 32;
-          uint32_t v[2][32];
-          tmem_ld_32x32b_x32(ta, v[0]);
+        const float sc = sc_lane[(it & (BG_SC - 1)) * 2 * BG_BM];
+        const bool more = kb + 1 < p.k_blocks;
+        const float2 s2 = pk2(sc, sc);
+        bool there = false;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            tmem_ld_wait(v[c & 1]);
-            if (c + 1 < NC) tmem_ld_32x32b_x32(ta + 32 * (c + 1), v[(c + 1) & 1]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 r = __ffma2_rn(pk2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2,
-                                          pk2(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]));
-              acc[32 * c + 2 * i] = r.x; acc[32 * c + 2 * i + 1] = r.y;
+        for (int c = 0; c < CW / 32; ++c) {
+          tmem_ld_wait(v[c & 1]);
+          if (c + 1 < CW / 32) {
+            tmem_ld_32x32b_x32(t_lane + (it & 1) * BN + 32 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_remote_relaxed(release_addr + 8 * (it & 1));
+            ++it;
+            there = more && __all_sync(0xffffffffu, mbar_test_wait(&acc_full[it & 1], (it >> 1) & 1));
+            if (there) {
+              tc_fence_after();
+              tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
             }
           }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 r = __ffma2_rn(pk2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2,
+                                        pk2(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]));
+            acc[32 * c + 2 * i] = r.x; acc[32 * c + 2 * i + 1] = r.y;
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[as]);
-        if (++as == ACC) { as = 0; aph ^= 1; }
+        if (more && !there) {
+          ok = stage_there();
+          if (!ok) break;
+          tc_fence_after();
+          tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
+        }
       }
       if (!ok || !live) continue;
       // 32 columns at a time.  Boxes of 32 rows x 128 bytes (32 columns of fp32, 64 of 16 bits) in the 128-byte swizzle.
@@ -189,8 +257,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }
           continue;
         }
+        uint8_t* const out_buf = smem + BG_OUT + e * BG_OUT_BUF + (f32 ? b & 1 : b >> 1) * (BG_OUT_BUF / 2);
         if (f32 || (b & 1) == 0) {
-          if (lane == 0) tma_store_wait_read<0>();           // the previous box has left the buffer
+          if (lane == 0) tma_store_wait_read<1>();           // the box before the previous one has left the buffer
           __syncwarp();
         }
         if (f32) {
@@ -206,7 +275,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             for (int j = 0; j < 4; ++j) {
               const float lo = acc[32 * b + 8 * pc + 2 * j], hi = acc[32 * b + 8 * pc + 2 * j + 1];
               if (p.c_type == GSB200_F16) w[j] = pack_half2(lo, hi);
-              else { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); w[j] = *reinterpret_cast<const uint32_t*>(&h); }
+              else w[j] = pack_bf2(lo, hi);
             }
             *reinterpret_cast<uint4*>(out_buf + lane * 128 + (((4 * (b & 1) + pc) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -221,26 +290,221 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     if (lane == 0) tma_store_wait_all<0>();
   }
   tc_fence_before();
+  // neither CTA leaves (or frees tensor memory) while the other may still arrive at its barriers or its MMAs write here
+  cluster_sync_all();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem_base, ACC * BN); }
+}
+
+// ---- few tiles ---------------------------------------------------------------------------------------------------------
+// One tile of 128 rows x BN columns per CTA.  With few rows the time is a chain of latencies: the narrow tile spreads the weight over the SMs,
+// and a K block takes BN tensor-memory columns, so that up to 512 / BN of them are multiplied before the first has been added.
+//   warp 0 TMA producer, warp 1 MMA issue, warps 2..9 epilogue (lane quarter w % 4, column half), results straight from registers
+constexpr int BS_THREADS = 32 * 10;
+template <int BN>
+struct BsSmem {
+  static constexpr int STAGE = BG_A_BYTES + BN * BG_BK;                    // 20, 24 or 32 KiB
+  static constexpr int STAGES = BN == 128 ? 6 : 8;
+  static constexpr int ACC = 512 / BN;                                     // tensor-memory stages: 16, 8, 4
+  static constexpr int BAR = STAGES * STAGE;
+  static constexpr int BYTES = BAR + (2 * STAGES + 2 * ACC) * 8 + 16 + 1024;
+  static_assert(BYTES <= 227 * 1024, "shared memory budget");
+};
+
+template <int BN, bool KN>
+__global__ void __launch_bounds__(BS_THREADS, 1)
+block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const BgParams p) {
+  extern __shared__ uint8_t bs_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(bs_smem_raw) + 1023) & ~uintptr_t(1023));
+  using L = BsSmem<BN>;
+  constexpr int STAGES = L::STAGES, ACC = L::ACC, CW = BN / 2;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + ACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACC);
+  const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m0 = (int)(blockIdx.x / p.n_blocks) * BG_BM, n0 = (int)(blockIdx.x % p.n_blocks) * BN;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < ACC; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], BG_EPI_WARPS); }
+    abort_flag.set(0);
+    fence_mbar_init();
+    prefetch_tmap(&tm_a); prefetch_tmap(&tm_b);
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
   __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, ACC * BN); }
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();                                           // (after the tensor memory is in hand: see launch_gemm_small)
+  pdl_wait();
+  const unsigned int budget = spin_budget();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int s = 0; uint32_t ph = 0;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE50 | s, budget)) { ok = false; break; }
+        uint8_t* st = smem + s * L::STAGE;
+        mbar_arrive_expect_tx(&full[s], L::STAGE);
+        tma_load_2d(st, &tm_a, &full[s], kb * BG_BK, m0);
+        if constexpr (KN) tma_load_2d(st + BG_A_BYTES, &tm_b, &full[s], n0, kb * BG_BK);
+        else tma_load_2d(st + BG_A_BYTES, &tm_b, &full[s], kb * BG_BK, n0);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+      if (!ok) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma_idesc(1, 0, 0, BG_BM, BN) | (KN ? UMMA_B_MN : 0u);
+    int s = 0, as = 0; uint32_t ph = 0, aph = 0;
+    for (int kb = 0; kb < p.k_blocks; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait<true>(&full[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xE60 | s, budget))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE70 | as, budget))) break;
+      tc_fence_after();
+      const uint32_t st = smem_u32(smem + s * L::STAGE);
+      const uint64_t a_desc = umma_smem_desc_sw128(st);
+      const uint64_t b_desc = KN ? umma_smem_desc_mn<BN>(st + BG_A_BYTES, 0) : umma_smem_desc_sw128(st + BG_A_BYTES);
+      constexpr uint64_t b_step = KN ? (32 * BN) >> 4 : 2;                  // K = 32: 32 rows of BN bytes, or 32 bytes of a row
+#pragma unroll
+      for (int k = 0; k < 4; ++k) umma_f8_elect(tmem_base + as * BN, a_desc + 2 * k, b_desc + b_step * k, idesc, k != 0);
+      umma_commit_elect(&acc_full[as]);
+      umma_commit_elect(&empty[s]);
+      if (++s == STAGES) { s = 0; ph ^= 1; }
+      if (++as == ACC) { as = 0; aph ^= 1; }
+    }
+  } else {
+    const int q = warp & 3, half = warp >= 6 ? 1 : 0;      // warps 2..5 and 6..9: each quarter once
+    const int row = m0 + q * 32 + lane, n = n0 + half * CW;
+    const bool live = m0 + q * 32 < p.M && n < p.N;
+    const float* sa = p.sa + (long long)(row < p.M ? row : p.M - 1) * p.ld_sa;
+    const float* sb = p.sb + (long long)((n < p.N ? n : 0) >> 7) * p.ld_sb_n;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + half * CW;
+    constexpr int AHEAD = 4;                               // scales are loaded so many K blocks ahead
+    float sc[AHEAD], sd[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      sc[j] = j < p.k_blocks ? ldg_f_here(sa + j) : 0.f;
+      sd[j] = j < p.k_blocks ? ldg_f_here(sb + (long long)j * p.ld_sb_k) : 0.f;
+    }
+    float acc[CW];
+#pragma unroll
+    for (int i = 0; i < CW; ++i) acc[i] = 0.f;
+    bool ok = true;
+    int as = 0; uint32_t aph = 0;
+    for (int kb0 = 0; ok && kb0 < p.k_blocks; kb0 += AHEAD) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int kb = kb0 + j;
+        if (kb >= p.k_blocks) break;
+        const float s1 = sc[j] * sd[j];
+        if (kb + AHEAD < p.k_blocks) {
+          sc[j] = ldg_f_here(sa + kb + AHEAD);
+          sd[j] = ldg_f_here(sb + (long long)(kb + AHEAD) * p.ld_sb_k);
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[as], aph, abort_flag, ST_TIMEOUT_EPILOGUE, 0xE80 | as, budget));
+        if (!ok) break;
+        tc_fence_after();
+        constexpr int CH = CW < 32 ? 16 : 32;
+#pragma unroll
+        for (int c = 0; c < CW / CH; ++c) {
+          uint32_t v[CH];
+          if constexpr (CH == 16) tmem_ld_32x32b_x16(t_lane + as * BN + CH * c, v);
+          else tmem_ld_32x32b_x32(t_lane + as * BN + CH * c, v);
+          tmem_ld_wait(v);
+          if (c + 1 == CW / CH) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&acc_empty[as]);
+          }
+#pragma unroll
+          for (int i = 0; i < CH; ++i) acc[CH * c + i] = fmaf(__uint_as_float(v[i]), s1, acc[CH * c + i]);
+        }
+        if (++as == ACC) { as = 0; aph ^= 1; }
+      }
+    }
+    if (ok && live && row < p.M) {
+      const int esz = p.c_type == GSB200_F32 ? 4 : 2;
+      uint8_t* dst = static_cast<uint8_t*>(p.C) + ((long long)row * p.ldc + n) * esz;
+      const bool wide = ((reinterpret_cast<uintptr_t>(p.C) | (uintptr_t)(p.ldc * esz)) & 31) == 0;
+      if (p.c_type == GSB200_F32) {
+#pragma unroll
+        for (int b = 0; b < CW / 8; ++b) {
+          if (wide && n + 8 * b + 8 <= p.N) {
+            stg_v8(dst + 32 * b, make_uint4(__float_as_uint(acc[8 * b]), __float_as_uint(acc[8 * b + 1]), __float_as_uint(acc[8 * b + 2]), __float_as_uint(acc[8 * b + 3])),
+                   make_uint4(__float_as_uint(acc[8 * b + 4]), __float_as_uint(acc[8 * b + 5]), __float_as_uint(acc[8 * b + 6]), __float_as_uint(acc[8 * b + 7])));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + 8 * b + i < p.N) reinterpret_cast<float*>(dst)[8 * b + i] = acc[8 * b + i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < CW / 16; ++b) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = p.c_type == GSB200_F16 ? pack_half2(acc[16 * b + 2 * i], acc[16 * b + 2 * i + 1]) : pack_bf2(acc[16 * b + 2 * i], acc[16 * b + 2 * i + 1]);
+          if (wide && n + 16 * b + 16 <= p.N) {
+            stg_v8(dst + 32 * b, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n + 16 * b + i < p.N) reinterpret_cast<uint16_t*>(dst)[16 * b + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
 template <int BN, bool KN>
-static cudaError_t launch_bg(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const BgParams& p, int dev, cudaStream_t st) {
+static cudaError_t launch_bs(const CUtensorMap& ta, const CUtensorMap& tb, const BgParams& p, int dev, int grid, cudaStream_t st) {
   static std::atomic<int> attr_done[64];
-  auto k = block_gemm_kernel<BN, KN>;
+  auto k = block_gemm_small_kernel<BN, KN>;
   if (!attr_done[dev].load(std::memory_order_acquire)) {
-    // the re-split of the registers waits until the block's own pool covers it
-    cudaFuncAttributes fa{};
-    cudaError_t e = cudaFuncGetAttributes(&fa, k);
-    if (e == cudaSuccess && fa.numRegs * BG_THREADS < 32 * (BG_FRONT_WARPS * 56 + BG_EPI_WARPS * 224)) e = cudaErrorInvalidConfiguration;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BgSmem<BN>::BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BsSmem<BN>::BYTES);
     if (e != cudaSuccess) return e;
     attr_done[dev].store(1, std::memory_order_release);
   }
-  const long long tiles = (long long)p.m_blocks * p.n_blocks;
-  const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
-  return launch_dependent(k, (unsigned)grid, BG_THREADS, (size_t)BgSmem<BN>::BYTES, st, ta, tb, tc, p);
+  return launch_dependent(k, (unsigned)grid, BS_THREADS, (size_t)BsSmem<BN>::BYTES, st, ta, tb, p);
+}
+
+// Launches `units` pairs; units = 0 asks how many can be resident (0: this form must not be launched here).
+template <bool KN>
+static cudaError_t launch_bg(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const BgParams& p, int dev, int units, int* capacity,
+                             cudaStream_t st) {
+  static std::atomic<int> cap[64];
+  auto k = block_gemm_kernel<KN>;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(BG_THREADS); cfg.dynamicSmemBytes = BG_BYTES; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  int c = cap[dev].load(std::memory_order_acquire);
+  if (c == 0) {
+    // the re-split of the registers waits until the block's own pool covers it
+    cudaFuncAttributes fa{};
+    cudaError_t e = cudaFuncGetAttributes(&fa, k);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BG_BYTES);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3((unsigned)(sm_count_physical() / 2 * 2));
+    int n = 0;
+    const bool pool = fa.numRegs * BG_THREADS >= 32 * (BG_FRONT_WARPS * BG_FRONT_REGS + BG_EPI_WARPS * BG_EPI_REGS) && fa.numRegs * BG_THREADS <= 65536;
+    c = pool && cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0 ? n : -1;
+    (void)cudaGetLastError();
+    cap[dev].store(c, std::memory_order_release);
+  }
+  if (units == 0) { *capacity = c > 0 ? c : 0; return cudaSuccess; }
+  cfg.gridDim = dim3((unsigned)(2 * units));
+  return cudaLaunchKernelEx(&cfg, k, ta, tb, tc, p);
 }
 
 int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb, const float* sb,
@@ -260,25 +524,54 @@ int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return GSB200_ERR_DEVICE;
-  constexpr int BN = 256;
+  CUtensorMap ta, tb, tc;
   BgParams p{};
-  p.M = (int)M; p.N = N; p.m_blocks = (int)((M + BG_BM - 1) / BG_BM); p.n_blocks = (N + BN - 1) / BN; p.k_blocks = kb;
-  if ((long long)p.m_blocks * p.n_blocks > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
+  p.M = (int)M; p.N = N; p.k_blocks = kb;
   p.sa = sa; p.ld_sa = ld_sa; p.sb = sb; p.ld_sb_n = kn ? 1 : ld_sb; p.ld_sb_k = kn ? ld_sb : 1;
   p.C = C; p.ldc = ldc; p.c_type = c_type;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  if (!tmap_2d(&ta, u8, 1, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BG_BK, BG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
+  const int sms = sm_count();
+  const long long rb = (M + BG_BM - 1) / BG_BM;
+  int bn = 0;                                                // the narrowest tile of which all are resident at once; none: pairs
+  for (int w = 32; w <= 128 && bn == 0; w *= 2)
+    if (rb * ((N + w - 1) / w) <= sms) bn = w;
+  int units = 0;
+  if (bn == 0) {
+    int cap = 0;
+    const cudaError_t e = kn ? launch_bg<true>(ta, ta, ta, p, dev, 0, &cap, st) : launch_bg<false>(ta, ta, ta, p, dev, 0, &cap, st);
+    if (e != cudaSuccess) return cuda_status(e, "block-scaled gemm set-up");
+    units = sms / 2 < cap ? sms / 2 : cap;
+    if (units == 0) bn = 128;
+  }
+  if (bn != 0) {
+    p.m_blocks = (int)rb; p.n_blocks = (N + bn - 1) / bn;
+    const long long tiles = rb * p.n_blocks;
+    if (tiles > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
+    const CUtensorMapSwizzle sw = bn == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bn == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    if (kn ? !tmap_2d(&tb, u8, 1, B, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, (uint32_t)bn, BG_BK, sw)
+           : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, (uint32_t)bn, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
+    const int g = (int)tiles;
+    const cudaError_t e = bn == 32 ? (kn ? launch_bs<32, true>(ta, tb, p, dev, g, st) : launch_bs<32, false>(ta, tb, p, dev, g, st))
+                        : bn == 64 ? (kn ? launch_bs<64, true>(ta, tb, p, dev, g, st) : launch_bs<64, false>(ta, tb, p, dev, g, st))
+                                   : (kn ? launch_bs<128, true>(ta, tb, p, dev, g, st) : launch_bs<128, false>(ta, tb, p, dev, g, st));
+    return cuda_status(e, "block-scaled gemm launch");
+  }
+  p.m_blocks = (int)((M + 2 * BG_BM - 1) / (2 * BG_BM)); p.n_blocks = (N + BG_BN - 1) / BG_BN;
+  const long long tiles = (long long)p.m_blocks * p.n_blocks;
+  if (tiles > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
   // TMA writes whole 16-byte pieces: where a row of C ends inside one, the last box goes element by element
   const bool tma_out = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * esz) % 16 == 0;
   p.n_tma = !tma_out ? 0 : (N * esz) % 16 == 0 ? N : N / (128 / esz) * (128 / esz);
-  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   const CUtensorMapDataType ct = c_type == GSB200_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                : c_type == GSB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap ta, tb, tc;
-  if (!tmap_2d(&ta, u8, 1, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BG_BK, BG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   if (kn ? !tmap_2d(&tb, u8, 1, B, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, 128, BG_BK, CU_TENSOR_MAP_SWIZZLE_128B)
-         : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, BN, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
+         : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   if (p.n_tma == 0) tc = ta;
   else if (!tmap_2d(&tc, ct, esz, C, (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 128 / esz, 32, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
-  return cuda_status(kn ? launch_bg<BN, true>(ta, tb, tc, p, dev, st) : launch_bg<BN, false>(ta, tb, tc, p, dev, st), "block-scaled gemm launch");
+  if (tiles < units) units = (int)tiles;
+  return cuda_status(kn ? launch_bg<true>(ta, tb, tc, p, dev, units, nullptr, st) : launch_bg<false>(ta, tb, tc, p, dev, units, nullptr, st),
+                     "block-scaled gemm launch");
 }
 
 }  // namespace gsb

@@ -157,6 +157,23 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t local_addr, uint32_t ra
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// ... without any ordering of memory, for hand-overs of tensor memory alone, from a loop that such an arrival is part of the chain of
+// (the default form waits for the thread's stores first).
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// One look at a barrier, which does not suspend the thread.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -286,16 +303,18 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
-// The same for an operand whose rows are the reduction ("MN-major"): rows of 128 bytes along M or N with the 128-byte swizzle (a TMA
-// box of 128 bytes x rows), 8-row groups 1024 bytes apart (SBO), the next 128 bytes along M or N `lbo` bytes further (LBO).  Advancing
-// along K by r rows = adding r * 128 >> 4.  The instruction descriptor says which operand is one (UMMA_A_MN, UMMA_B_MN).
+// The same for an operand whose rows are the reduction ("MN-major"): rows of W = 32, 64 or 128 bytes along M or N in the swizzle of that width
+// (a TMA box of W bytes x rows), 8-row groups 8 W bytes apart (SBO), the next W bytes along M or N `lbo` bytes further (LBO).
+// Advancing along K by r rows = adding r * W >> 4.  The instruction descriptor says which operand is one (UMMA_A_MN, UMMA_B_MN).
+template <int W>
 __device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t smem_addr, uint32_t lbo) {
+  static_assert(W == 32 || W == 64 || W == 128, "swizzle width");
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
   d |= (uint64_t)(lbo >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)((8 * W) >> 4) << 32;
   d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
+  d |= (uint64_t)(W == 128 ? 2 : W == 64 ? 4 : 6) << 61;
   return d;
 }
 constexpr uint32_t UMMA_A_MN = 1u << 15, UMMA_B_MN = 1u << 16;
@@ -392,6 +411,18 @@ __device__ __forceinline__ void umma_commit_pair_both(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                ::"r"(smem_u32(bar)), "h"((uint16_t)3)
                : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair_both_elect(uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+               "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+               ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // The forms for a CONVERGED warp, of which one elected lane issues the instruction: the operands stay in uniform registers
 // across the loop around it, where a single thread moves them there for every MMA.

@@ -122,7 +122,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
           !__all_sync(0xffffffffu, mbar_wait(&full_b[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF20 | s, budget))) { ok = false; break; }
       tc_fence_after();
       const uint32_t st = smem_u32(smem + s * WG_STAGE);
-      const uint64_t a_desc = umma_smem_desc_mn(st, WG_CHUNK), b_desc = umma_smem_desc_mn(st + WG_A_BYTES, WG_CHUNK);
+      const uint64_t a_desc = umma_smem_desc_mn<128>(st, WG_CHUNK), b_desc = umma_smem_desc_mn<128>(st + WG_A_BYTES, WG_CHUNK);
       constexpr uint64_t step = (16 * 128) >> 4;           // K = 16: 16 rows of 128 bytes
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
