@@ -82,7 +82,9 @@ NATIVE_ENTRIES = ["gsb200_ptq_int8", "gsb200_ptq_fp8", "gsb200_ptq_mxfp8", "gsb2
                   "gsb200_gemm_i8_rotary_f16", "gsb200_gemm_fp8_rotary_f16", "gsb200_dual_gemm_i8_silu_f16",
                   "gsb200_dual_gemm_fp8_silu_f16", "gsb200_dual_gemm_fp8_silu_mxfp8", "gsb200_mx_tiled_scale_bytes",
                   "gsb200_mx_scales_to_tiled", "gsb200_gemm_mxfp8_f16", "gsb200_dual_gemm_mxfp8_silu_f16",
-                  "gsb200_fac_gemm_fp8_f16", "gsb200_factored_lstm_step"]
+                  "gsb200_fac_gemm_fp8_f16", "gsb200_factored_lstm_step", "gsb200_block_quantize_fp8", "gsb200_block_dequantize_fp8",
+                  "gsb200_gemm_fp8_block", "gsb200_gemm_fp8_block_wgrad_workspace_bytes", "gsb200_gemm_fp8_block_wgrad", "gsb200_swiglu_fp8_block",
+                  "gsb200_swiglu_fp8_block_bwd"]
 
 
 def lib():

@@ -28,7 +28,7 @@ namespace {
 
 // Entry points of the loaded library, handed over as addresses (the ctypes handle owns the library).
 enum Entry { PTQ_INT8, PTQ_FP8, PTQ_MXFP8, GEMM_I8, GEMM_FP8, ROT_I8, ROT_FP8, DUAL_I8, DUAL_FP8, DUAL_FP8_MX, MX_BYTES, MX_TILE, MX_GEMM,
-             MX_DUAL, FAC_GEMM, FAC_STEP, N_ENTRIES };
+             MX_DUAL, FAC_GEMM, FAC_STEP, BLOCK_QUANT, BLOCK_DEQUANT, BLOCK_GEMM, BLOCK_WGRAD_BYTES, BLOCK_WGRAD, BLOCK_SWIGLU, BLOCK_SWIGLU_BWD, N_ENTRIES };
 void* g_entry[N_ENTRIES];
 PyObject* g_check;             // check(status, what), raises
 template <typename Fn>
@@ -75,7 +75,26 @@ struct Call {
     if (direct) return at::Tensor(at::detail::empty_cuda(size, dt, device, std::nullopt));
     return at::empty(size, at::TensorOptions().device(device).dtype(dt));
   }
+  // [m, n] with rows on 16-byte boundaries
+  at::Tensor empty_rows(int64_t m, int64_t n, at::ScalarType dt) {
+    const int64_t per = 16 / (int64_t)c10::elementSize(dt), ld = (n + per - 1) / per * per;
+    if (ld == n) return empty({m, n}, dt);
+    return at::empty_strided({m, n}, {ld, 1}, at::TensorOptions().device(device).dtype(dt));
+  }
 };
+
+// Block-scaled FP8: what ops.py's checks ask of a tensor, and its output layout (rows on 16-byte boundaries).
+constexpr int64_t BLOCK = 128;
+int64_t blocks(int64_t n) { return (n + BLOCK - 1) / BLOCK; }
+bool block_dt(at::ScalarType t, int32_t& dt) {
+  dt = t == at::kHalf ? GSB200_F16 : t == at::kBFloat16 ? GSB200_BF16 : t == at::kFloat ? GSB200_F32 : -1;
+  return dt >= 0;
+}
+bool shaped(const at::Tensor* t, int64_t m, int64_t n) {
+  return t->dim() == 2 && t->size(0) == m && t->size(1) == n && m > 0 && n > 0 && n <= (1 << 30) && (n == 1 || t->stride(1) == 1) && (m == 1 || t->stride(0) >= n);
+}
+bool any_shape(const at::Tensor* t) { return t->dim() == 2 && shaped(t, t->size(0), t->size(1)); }
+int64_t ld(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
 
 bool modes_active() { return c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled(); }
 
@@ -335,6 +354,108 @@ OPERATOR(fac_step, 8)
   Py_RETURN_TRUE;
 OPERATOR_END
 
+// (x, rows, out, out_scale)
+OPERATOR(block_quantize, 4)
+  const at::Tensor *x, *q0, *s0;
+  int32_t rows, dt;
+  SLOW_UNLESS(c.tensor(a[0], x) && int32(a[1], rows) && (rows == 1 || rows == BLOCK) && c.optional(a[2], q0) && c.optional(a[3], s0));
+  SLOW_UNLESS(any_shape(x) && block_dt(x->scalar_type(), dt));
+  const int64_t M = x->size(0), K = x->size(1), sm = rows == 1 ? M : blocks(M), sk = blocks(K);
+  SLOW_UNLESS((!q0 || (is_f8(q0) && shaped(q0, M, K))) && (!s0 || (s0->scalar_type() == at::kFloat && shaped(s0, sm, sk))));
+  const at::Tensor q = q0 ? *q0 : c.empty_rows(M, K, at::kFloat8_e4m3fn);
+  const at::Tensor s = s0 ? *s0 : c.empty({sm, sk}, at::kFloat);
+  CHECK(call(ENTRY(BLOCK_QUANT, gsb200_block_quantize_fp8), x->data_ptr(), dt, ld(*x), ptr<uint8_t>(q), ld(q), ptr<float>(s), ld(s), M, (int32_t)K, rows,
+             c.stream()), "fp8_block_quantize");
+  return pair(result(a[2], q), result(a[3], s));
+OPERATOR_END
+
+// An E4M3 tensor and its scales
+bool f8_scaled(const at::Tensor* q, const at::Tensor* s, int64_t rows) {
+  return any_shape(q) && is_f8(q) && s->scalar_type() == at::kFloat && shaped(s, rows == 1 ? q->size(0) : blocks(q->size(0)), blocks(q->size(1)));
+}
+
+// (q, scale, rows, dtype code, out)
+OPERATOR(block_dequantize, 5)
+  const at::Tensor *q, *s, *x0;
+  int32_t rows, code;
+  SLOW_UNLESS(c.tensor(a[0], q) && c.tensor(a[1], s) && int32(a[2], rows) && (rows == 1 || rows == BLOCK) && int32(a[3], code) && c.optional(a[4], x0));
+  SLOW_UNLESS(f8_scaled(q, s, rows));
+  const int64_t M = q->size(0), K = q->size(1);
+  SLOW_UNLESS(x0 ? shaped(x0, M, K) && block_dt(x0->scalar_type(), code) : code >= 0 && code <= 2);
+  const at::Tensor x = x0 ? *x0 : c.empty_rows(M, K, code == GSB200_F16 ? at::kHalf : code == GSB200_BF16 ? at::kBFloat16 : at::kFloat);
+  CHECK(call(ENTRY(BLOCK_DEQUANT, gsb200_block_dequantize_fp8), ptr<uint8_t>(q), ld(*q), ptr<float>(s), ld(*s), x.data_ptr(), code, ld(x), M, (int32_t)K, rows,
+             c.stream()), "fp8_block_dequantize");
+  return result(a[4], x);
+OPERATOR_END
+
+// (A, B, scale_a, scale_b, out, dtype code, b_transposed)
+OPERATOR(block_gemm, 7)
+  const at::Tensor *A, *B, *sa, *sb, *C0;
+  int32_t code;
+  SLOW_UNLESS(c.tensor(a[0], A) && c.tensor(a[1], B) && c.tensor(a[2], sa) && c.tensor(a[3], sb) && c.optional(a[4], C0) && int32(a[5], code) && PyBool_Check(a[6]));
+  const bool kn = a[6] == Py_True;
+  SLOW_UNLESS(f8_scaled(A, sa, 1) && f8_scaled(B, sb, BLOCK));
+  const int64_t M = A->size(0), K = A->size(1), N = B->size(kn ? 1 : 0);
+  SLOW_UNLESS(B->size(kn ? 0 : 1) == K && (C0 ? shaped(C0, M, N) && block_dt(C0->scalar_type(), code) : code >= 0 && code <= 2));
+  const at::Tensor C = C0 ? *C0 : c.empty_rows(M, N, code == GSB200_F16 ? at::kHalf : code == GSB200_BF16 ? at::kBFloat16 : at::kFloat);
+  CHECK(call(ENTRY(BLOCK_GEMM, gsb200_gemm_fp8_block), ptr<uint8_t>(A), ld(*A), ptr<float>(sa), ld(*sa), ptr<uint8_t>(B), ld(*B), ptr<float>(sb), ld(*sb),
+             C.data_ptr(), ld(C), code, M, (int32_t)N, (int32_t)K, kn ? GSB200_FLAG_B_KN : 0, c.stream()), "gemm_fp8_block");
+  return result(a[4], C);
+OPERATOR_END
+
+// (dy, q, scale, out, accumulate)
+OPERATOR(block_wgrad, 5)
+  const at::Tensor *dy, *q, *s, *w0;
+  int32_t dt;
+  SLOW_UNLESS(c.tensor(a[0], dy) && c.tensor(a[1], q) && c.tensor(a[2], s) && c.optional(a[3], w0) && PyBool_Check(a[4]));
+  const bool acc = a[4] == Py_True;
+  SLOW_UNLESS(any_shape(dy) && block_dt(dy->scalar_type(), dt) && dt != GSB200_F32 && f8_scaled(q, s, 1) && q->size(0) == dy->size(0) && (w0 || !acc));
+  const int64_t M = dy->size(0), N = dy->size(1), K = q->size(1);
+  SLOW_UNLESS(!w0 || (w0->scalar_type() == at::kFloat && shaped(w0, N, K)));
+  const at::Tensor w = w0 ? *w0 : c.empty({N, K}, at::kFloat);
+  const int64_t need = ENTRY(BLOCK_WGRAD_BYTES, gsb200_gemm_fp8_block_wgrad_workspace_bytes)(M, (int32_t)N, (int32_t)K);
+  at::Tensor ws;
+  if (need > 0) ws = c.empty({need}, at::kByte);
+  CHECK(call(ENTRY(BLOCK_WGRAD, gsb200_gemm_fp8_block_wgrad), dy->data_ptr(), dt, ld(*dy), ptr<uint8_t>(q), ld(*q), ptr<float>(s), ld(*s), ptr<float>(w), ld(w),
+             acc ? 1 : 0, need > 0 ? ws.data_ptr() : nullptr, need, M, (int32_t)N, (int32_t)K, c.stream()), "gemm_fp8_block_wgrad");
+  return result(a[3], w);
+OPERATOR_END
+
+// (gate, up) -> ((h, scale), (gate, scale), (up, scale))
+OPERATOR(block_swiglu, 2)
+  const at::Tensor *g, *u;
+  int32_t dt;
+  SLOW_UNLESS(c.tensor(a[0], g) && c.tensor(a[1], u) && any_shape(g) && block_dt(g->scalar_type(), dt) && u->scalar_type() == g->scalar_type());
+  const int64_t M = g->size(0), F = g->size(1);
+  SLOW_UNLESS(shaped(u, M, F));
+  at::Tensor q[3], s[3];
+  for (int i = 0; i < 3; ++i) { q[i] = c.empty_rows(M, F, at::kFloat8_e4m3fn); s[i] = c.empty({M, blocks(F)}, at::kFloat); }
+  CHECK(call(ENTRY(BLOCK_SWIGLU, gsb200_swiglu_fp8_block), g->data_ptr(), ld(*g), u->data_ptr(), ld(*u), dt, ptr<uint8_t>(q[0]), ptr<float>(s[0]), ptr<uint8_t>(q[1]),
+             ptr<float>(s[1]), ptr<uint8_t>(q[2]), ptr<float>(s[2]), q[0].stride(0), s[0].stride(0), M, (int32_t)F, c.stream()), "swiglu_fp8_block");
+  PyObject* r = PyTuple_New(3);
+  for (int i = 0; r && i < 3; ++i) {
+    PyObject* p = pair(wrap(q[i]), wrap(s[i]));
+    if (!p) { Py_DECREF(r); return nullptr; }
+    PyTuple_SET_ITEM(r, i, p);
+  }
+  return r;
+OPERATOR_END
+
+// (dh, gate_q, gate_scale, up_q, up_scale) -> (dgate, dup)
+OPERATOR(block_swiglu_bwd, 5)
+  const at::Tensor *d, *gq, *gs, *uq, *us;
+  int32_t dt;
+  SLOW_UNLESS(c.tensor(a[0], d) && c.tensor(a[1], gq) && c.tensor(a[2], gs) && c.tensor(a[3], uq) && c.tensor(a[4], us));
+  SLOW_UNLESS(any_shape(d) && block_dt(d->scalar_type(), dt) && f8_scaled(gq, gs, 1) && f8_scaled(uq, us, 1) && gq->sizes() == d->sizes() && uq->sizes() == d->sizes());
+  const int64_t M = d->size(0), F = d->size(1);
+  const at::Tensor dg = c.empty_rows(M, F, d->scalar_type()), du = c.empty_rows(M, F, d->scalar_type());
+  CHECK(call(ENTRY(BLOCK_SWIGLU_BWD, gsb200_swiglu_fp8_block_bwd), d->data_ptr(), dt, ld(*d), ptr<uint8_t>(gq), ld(*gq), ptr<float>(gs), ld(*gs), ptr<uint8_t>(uq),
+             ld(*uq), ptr<float>(us), ld(*us), dg.data_ptr(), dg.stride(0), du.data_ptr(), du.stride(0), (uint8_t*)nullptr, (float*)nullptr, (uint8_t*)nullptr,
+             (float*)nullptr, (int64_t)0, (int64_t)0, M, (int32_t)F, c.stream()), "swiglu_fp8_block_bwd");
+  return pair(wrap(dg), wrap(du));
+OPERATOR_END
+
+
 // bind(addresses, check): the entry points' addresses in the order of `Entry`, and what turns a status into an exception
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *seq, *check;
@@ -360,6 +481,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, METHOD(quantize), METHOD(quantize_mx), METHOD(gemm), METHOD(rotary), METHOD(dual),
                          METHOD(dual_mx), METHOD(mx_tile), METHOD(mx_gemm), METHOD(mx_dual), METHOD(fac_gemm), METHOD(fac_step),
+                         METHOD(block_quantize), METHOD(block_dequantize), METHOD(block_gemm), METHOD(block_wgrad), METHOD(block_swiglu), METHOD(block_swiglu_bwd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -510,8 +510,7 @@ def _rows16(m, n, dtype, device):
     """An [m, n] output whose rows start on 16-byte boundaries: what the tensor cores read, and the fast stores."""
     per = 16 // dtype.itemsize
     ld = (n + per - 1) // per * per
-    t = torch.empty((m, ld), dtype=dtype, device=device)
-    return t if ld == n else t[:, :n]
+    return torch.empty((m, n), dtype=dtype, device=device) if ld == n else torch.empty_strided((m, n), (ld, 1), dtype=dtype, device=device)
 
 
 def _given(t, shape, dtypes, name):
@@ -550,6 +549,11 @@ def fp8_block_quantize(x, rows=1, out=None, out_scale=None):
     gradients and checkpoints: scales [M, ceil(K/128)]) or per 128 x 128 tile (``rows=128``, weights: [ceil(M/128), ceil(K/128)]).
     Scales are the smallest powers of two with ``max|x| <= 448 * scale``.  The elements' rows start on 16-byte boundaries, as the
     products want them."""
+    n = _lib.native
+    if n is not None:
+        r = n.block_quantize(x, rows, out, out_scale)
+        if r is not None:
+            return r
     return _checked_fp8_block_quantize(x, rows, out, out_scale)
 
 
@@ -572,6 +576,11 @@ def _checked_fp8_block_quantize(x, rows, out, out_scale):
 def fp8_block_dequantize(q, scale, rows=1, dtype=torch.bfloat16, out=None):
     """The values ``q * scale`` of a block-scaled tensor as fp16, bf16 or fp32 (a checkpoint restored, for a backward pass of the
     caller's own).  Exact in bf16 and fp32 for scales that are powers of two."""
+    n = _lib.native
+    if n is not None:
+        r = n.block_dequantize(q, scale, rows, _BLOCK_DT.get(dtype, -1), out)
+        if r is not None:
+            return r
     return _checked_fp8_block_dequantize(q, scale, rows, dtype, out)
 
 
@@ -596,6 +605,11 @@ def gemm_fp8_block(A, B, scale_a, scale_b, out=None, dtype=torch.float16, b_tran
     """``A[M,K] . B[N,K]^T`` over block-scaled FP8 operands -> fp16, bf16 or fp32: ``scale_a`` [M, ceil(K/128)], ``scale_b``
     [ceil(N/128), ceil(K/128)].  ``b_transposed``: B is [K,N] with scales [ceil(K/128), ceil(N/128)], which is the input gradient
     ``dY . W`` with the weight as the forward pass has it.  Sums and scales in fp32, one rounding."""
+    n = _lib.native
+    if n is not None:
+        r = n.block_gemm(A, B, scale_a, scale_b, out, _BLOCK_DT.get(dtype, -1), b_transposed)
+        if r is not None:
+            return r
     return _checked_gemm_fp8_block(A, B, scale_a, scale_b, out, dtype, b_transposed)
 
 
@@ -622,6 +636,11 @@ def _checked_gemm_fp8_block(A, B, scale_a, scale_b, out, dtype, b_transposed):
 def gemm_fp8_block_wgrad(dy, q, scale, out=None, accumulate=False):
     """Weight gradient ``dY^T . X`` [N,K] fp32 from ``dy`` [M,N] fp16/bf16 and the block-scaled 8-bit checkpoint ``q`` [M,K],
     ``scale`` [M, ceil(K/128)] of the layer's input.  ``accumulate`` adds to ``out``.  Rows of ``dy`` on 16-byte boundaries."""
+    n = _lib.native
+    if n is not None:
+        r = n.block_wgrad(dy, q, scale, out, accumulate)
+        if r is not None:
+            return r
     return _checked_gemm_fp8_block_wgrad(dy, q, scale, out, accumulate)
 
 
@@ -648,6 +667,11 @@ def _checked_gemm_fp8_block_wgrad(dy, q, scale, out, accumulate):
 def swiglu_fp8_block(gate, up):
     """``gate * sigmoid(gate) * up`` as a block-scaled FP8 tensor, with 8-bit checkpoints of both inputs: ``((h, scale), (gate, scale),
     (up, scale))``, each what ``fp8_block_quantize`` makes (of ``h``: from its fp32 values)."""
+    n = _lib.native
+    if n is not None:
+        r = n.block_swiglu(gate, up)
+        if r is not None:
+            return r
     return _checked_swiglu_fp8_block(gate, up)
 
 
@@ -669,6 +693,11 @@ def _checked_swiglu_fp8_block(gate, up):
 def swiglu_fp8_block_bwd(dh, gate_q, gate_scale, up_q, up_scale, quantize=False):
     """Gradients of SwiGLU from the checkpoints: ``(dgate, dup)`` in ``dh``'s type.  ``quantize``: also ``(q, scale)`` of each, as
     ``fp8_block_quantize`` makes of them, in the same pass: ``(dgate, dup, (q, scale), (q, scale))``."""
+    n = _lib.native
+    if n is not None and not quantize:
+        r = n.block_swiglu_bwd(dh, gate_q, gate_scale, up_q, up_scale)
+        if r is not None:
+            return r
     return _checked_swiglu_fp8_block_bwd(dh, gate_q, gate_scale, up_q, up_scale, quantize)
 
 

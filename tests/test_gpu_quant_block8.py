@@ -461,3 +461,51 @@ def test_offsets_beyond_32_bits():
     b, sb = g.fp8_block_quantize(rnd(gen, 16, k).cuda(), rows=128)
     c = g.gemm_fp8_block(q.view(F8), b, s, sb)
     assert torch.equal(c[-128:], g.gemm_fp8_block(q[-128:].view(F8), b, s[-128:], sb)) and bool((c[:-128] == 0).all())
+
+
+# ---- the native call path ----------------------------------------------------------------------------------------------------------
+def test_native_path_gives_the_bytes_of_the_checked_path():
+    """Every operator through csrc/binding.cpp and through its checked Python function, aligned and ragged widths, given outputs."""
+    g = need_lib()
+    from gigaslop_b200 import _lib, ops
+    n = _lib.native
+    assert n is not None
+    same = lambda a, b: a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype and torch.equal(a.view(torch.uint8) if a.dtype == F8 else a, b.view(torch.uint8) if b.dtype == F8 else b)
+    gen = torch.Generator().manual_seed(21)
+    for m, f, o in ((70, 256, 384), (33, 200, 72), (1, 128, 8), (5, 333, 130)):
+        x = rnd(gen, m, f).half().cuda()
+        for rows in (1, 128):
+            a, b = n.block_quantize(x, rows, None, None), ops._checked_fp8_block_quantize(x, rows, None, None)
+            assert same(a[0], b[0]) and same(a[1], b[1])
+            assert same(n.block_dequantize(*a, rows, _lib.BF16, None), ops._checked_fp8_block_dequantize(*b, rows, torch.bfloat16, None))
+        q, s = g.fp8_block_quantize(x)
+        for tr in (False, True):
+            w, sw = g.fp8_block_quantize(rnd(gen, *((f, o) if tr else (o, f))).cuda(), rows=128)
+            for code, dt in ((_lib.F16, torch.float16), (_lib.BF16, torch.bfloat16), (_lib.F32, torch.float32)):
+                assert same(n.block_gemm(q, w, s, sw, None, code, tr), ops._checked_gemm_fp8_block(q, w, s, sw, None, dt, tr))
+                out = torch.empty(m, o, dtype=dt, device="cuda")
+                assert n.block_gemm(q, w, s, sw, out, code, tr) is out and same(out, ops._checked_gemm_fp8_block(q, w, s, sw, torch.empty_like(out), dt, tr))
+        dy = rnd(gen, m, (o + 7) // 8 * 8).half().cuda()[:, :o]
+        assert same(n.block_wgrad(dy, q, s, None, False), ops._checked_gemm_fp8_block_wgrad(dy, q, s, None, False))
+        acc, acc2 = (torch.ones(o, f, device="cuda") for _ in range(2))
+        assert n.block_wgrad(dy, q, s, acc, True) is acc and same(acc, ops._checked_gemm_fp8_block_wgrad(dy, q, s, acc2, True))
+        a, b = n.block_swiglu(x, x), ops._checked_swiglu_fp8_block(x, x)
+        assert all(same(u, v) for p, r in zip(a, b) for u, v in zip(p, r))
+        a, b = n.block_swiglu_bwd(x, q, s, q, s), ops._checked_swiglu_fp8_block_bwd(x, q, s, q, s, False)
+        assert same(a[0], b[0]) and same(a[1], b[1])
+
+
+def test_native_path_leaves_the_rest_to_the_checked_path():
+    g = need_lib()
+    from gigaslop_b200 import _lib
+    n = _lib.native
+    z = lambda *sh, dt=torch.float16: torch.zeros(*sh, dtype=dt, device="cuda")
+    x, q, s, w, sw, dy = z(40, 256), z(40, 256, dt=torch.uint8), z(40, 2, dt=torch.float32), z(64, 256, dt=torch.uint8), z(1, 2, dt=torch.float32), z(40, 64)
+    for i, r in enumerate((n.block_quantize(x.t(), 1, None, None), n.block_quantize(x, 2, None, None), n.block_quantize(x[:0], 1, None, None), n.block_quantize(x.int(), 1, None, None),
+              n.block_quantize(x, 1, q[:, :8], None), n.block_quantize(x, 1, None, s[:, :1]),
+              n.block_dequantize(q, s[:, :1], 1, 0, None), n.block_dequantize(q, s, 128, 0, None), n.block_dequantize(q, s, 1, -1, None), n.block_dequantize(x, s, 1, 0, None),
+              n.block_gemm(q, w[:, :240], s, sw, None, 0, False), n.block_gemm(q, w, s, sw, None, 0, True), n.block_gemm(q, w, s, sw, None, -1, False), n.block_gemm(q, w, s, s, None, 0, False),
+              n.block_gemm(q, w, s, sw, x, 0, False), n.block_gemm(q, w, s, sw, None, 0, 0),
+              n.block_wgrad(dy.float(), q, s, None, False), n.block_wgrad(dy, q, s, None, True), n.block_wgrad(dy[:39], q, s, None, False), n.block_wgrad(dy, q, s, x, False),
+              n.block_swiglu(x, x[:, :128]), n.block_swiglu(x, x.float()), n.block_swiglu(x.cpu(), x), n.block_swiglu_bwd(x, q, s, q[:39], s), n.block_swiglu_bwd(x, q, s, q, s[:, :1]))):
+        assert r is None, i
