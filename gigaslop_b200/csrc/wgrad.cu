@@ -6,10 +6,12 @@
 // against a 16-bit copy of the checkpoint that never exists in memory.  (A scale that is no power of two rounds the product to dY's
 // type.)  The reduction runs over the rows of both operands, which the tensor core reads "MN-major".
 //
-// A CTA computes 256 x 256 of dW (two accumulators of 128 rows, all of TMEM) over a range of rows of the batch, 64 rows per step:
+// A CTA pair (cta_group::2) computes 512 x 256 of dW (two accumulators of 128 rows in each CTA, all of its tensor memory; narrow layers
+// 256 x 256, one accumulator) over a range of rows of the batch, 64 rows per step.  A CTA holds its own rows of dW, i.e. columns of dY, and half
+// of the tile's columns of x^, so an element of x^ is restored once per 512 columns of dY:
 //   warp 0      TMA producer: dY, boxes of 64 rows x 64 columns
-//   warp 1      MMA issue: 2 x 4 MMAs (M = 128, N = 256, K = 16) per step, 1024 tensor clocks
-//   warps 4..11 restore the step's 64 x 256 elements of x^ from global memory into the operand tile; at the end they write dW
+//   warp 1      MMA issue (first CTA): 4 MMAs (M = 256, N = 256, K = 16) per accumulator and step, 512 tensor clocks
+//   warps 4..11 restore the step's 64 x 128 elements of x^ from global memory into the operand tile; at the end they write dW
 // Few tiles are cut over the batch: each part writes its sums to the workspace, and a second launch adds them in order.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -21,16 +23,23 @@
 
 namespace gsb {
 
-constexpr int WG_BN = 256, WG_BK = 256, WG_BM = 64;        // columns of dY, columns of x^, rows per step
-constexpr int WG_A_BYTES = WG_BM * WG_BN * 2;              // 32 KiB
-constexpr int WG_B_BYTES = WG_BM * WG_BK * 2;              // 32 KiB
-constexpr int WG_STAGE = WG_A_BYTES + WG_B_BYTES;
-constexpr int WG_STAGES = 3;
-constexpr int WG_BAR = WG_STAGES * WG_STAGE;
-constexpr int WG_BYTES = WG_BAR + 256 + 1024;
+constexpr int WG_BK = 256, WG_BM = 64;                     // columns of x^ (a pair's), rows per step
 constexpr int WG_WARPS = 8, WG_FRONT = 4, WG_THREADS = 32 * (WG_WARPS + WG_FRONT);
 constexpr int WG_CHUNK = WG_BM * 128;                      // a 64-column chunk of an operand tile: 64 rows of 128 bytes
-static_assert(WG_BYTES <= 227 * 1024, "shared memory budget");
+// Steps that the tensor core sums by itself.  Its fp32 additions truncate: over 8192 rows the sums are off by some 3.5e-6 (2-norm; plain fp32 sums 2e-7),
+// and it grows with the rows; longer parts are added to dW every so many steps, in fp32 as the parts are.
+constexpr int WG_SEG = 128;
+constexpr int WG_AHEAD = 4;                                // steps of x^ in flight to the registers
+constexpr int WG_B_BYTES = 2 * WG_CHUNK;                   // a CTA's 128 columns of x^
+template <int ACC>                                         // accumulators (128 rows of dW per CTA each)
+struct WgSmem {
+  static constexpr int A_BYTES = ACC * 2 * WG_CHUNK;
+  static constexpr int STAGE = A_BYTES + WG_B_BYTES;       // 48 or 32 KiB
+  static constexpr int STAGES = ACC == 2 ? 4 : 6;
+  static constexpr int BAR = STAGES * STAGE;
+  static constexpr int BYTES = BAR + 256 + 1024;
+  static_assert(BYTES <= 227 * 1024, "shared memory budget");
+};
 
 struct WgParams {
   const uint8_t* q; long long ldq; const float* s; long long lds;
@@ -49,7 +58,7 @@ __device__ __forceinline__ void restore16<__half>(uint4 r, float s, uint4& lo, u
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3)));
-    o[i] = pack_half2(f.x * s, f.y * s);
+    o[i] = pack_half2_from(fmul2(f, make_float2(s, s)));
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]); hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
@@ -60,40 +69,49 @@ __device__ __forceinline__ void restore16<__nv_bfloat16>(uint4 r, float s, uint4
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3)));
-    const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * s, f.y * s);
-    o[i] = *reinterpret_cast<const uint32_t*>(&b);
+    const float2 v = fmul2(f, make_float2(s, s));
+    o[i] = pack_bf2(v.x, v.y);
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]); hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-template <typename T>
+// Sums of four floats held as words
+__device__ __forceinline__ uint4 add4(uint4 a, uint4 b) {
+  return make_uint4(__float_as_uint(__uint_as_float(a.x) + __uint_as_float(b.x)), __float_as_uint(__uint_as_float(a.y) + __uint_as_float(b.y)),
+                    __float_as_uint(__uint_as_float(a.z) + __uint_as_float(b.z)), __float_as_uint(__uint_as_float(a.w) + __uint_as_float(b.w)));
+}
+
+template <typename T, int ACC>
 __global__ void __launch_bounds__(WG_THREADS, 1)
 wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
   extern __shared__ uint8_t wg_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wg_smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_a = reinterpret_cast<uint64_t*>(smem + WG_BAR);
-  uint64_t* full_b = full_a + WG_STAGES;
-  uint64_t* empty = full_b + WG_STAGES;
-  uint64_t* acc_full = empty + WG_STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  using L = WgSmem<ACC>;
+  constexpr int STAGES = L::STAGES;
+  uint64_t* full_a = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* full_b = full_a + STAGES;
+  uint64_t* empty = full_b + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = (int)(blockIdx.x % p.tiles), part = (int)(blockIdx.x / p.tiles);
-  const int n0 = tile / p.k_tiles * WG_BN, k0 = tile % p.k_tiles * WG_BK;
+  const int rank = (int)cluster_ctarank();                 // the pair's first CTA issues the MMAs; its barriers collect both CTAs' operands
+  const int unit = (int)(blockIdx.x >> 1), tile = unit % p.tiles, part = unit / p.tiles;
+  const int n0 = tile / p.k_tiles * (256 * ACC) + rank * 128, k0 = tile % p.k_tiles * WG_BK;      // accumulator j: columns n0 + 256 j .. of dY
   const int step0 = (int)((long long)p.steps * part / p.parts), step1 = (int)((long long)p.steps * (part + 1) / p.parts);
-  const bool two = n0 + 128 < p.N;                         // the second accumulator has columns of dY
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WG_STAGES; ++s) { mbar_init(&full_a[s], 1); mbar_init(&full_b[s], WG_WARPS); mbar_init(&empty[s], 1); }
-    mbar_init(acc_full, 1);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_a[s], 1); mbar_init(&full_b[s], 2 * WG_WARPS); mbar_init(&empty[s], 1); }
+    mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS);
     abort_flag.set(0);
     fence_mbar_init();
     prefetch_tmap(&tm_dy);
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc_pair(tmem_slot, 256 * ACC); tmem_relinquish_pair(); }
   pdl_wait();
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();                                      // (a __syncthreads of both CTAs) the other's barriers are initialised before anything arrives at them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const unsigned int budget = spin_budget();
@@ -104,126 +122,168 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
       int s = 0; uint32_t ph = 0;
       for (int i = step0; i < step1; ++i) {
         if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xF00 | s, budget)) { ok = false; break; }
-        uint8_t* st = smem + s * WG_STAGE;
-        const int chunks = two ? 4 : 2;
-        mbar_arrive_expect_tx(&full_a[s], chunks * WG_CHUNK);
-        for (int j = 0; j < chunks; ++j) tma_load_2d(st + j * WG_CHUNK, &tm_dy, &full_a[s], n0 + 64 * j, i * WG_BM);
-        if (++s == WG_STAGES) { s = 0; ph ^= 1; }
+        uint8_t* st = smem + s * L::STAGE;
+        const uint32_t bar = mapa_shared(smem_u32(&full_a[s]), 0);
+        if (rank == 0) mbar_arrive_expect_tx(&full_a[s], 2 * L::A_BYTES);
+#pragma unroll
+        for (int j = 0; j < 2 * ACC; ++j) tma_load_2d_pair(st + j * WG_CHUNK, &tm_dy, bar, n0 + 256 * (j >> 1) + 64 * (j & 1), i * WG_BM);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
       }
       if (!ok) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t idesc = umma_idesc(1, fmt, fmt, 128, WG_BK) | UMMA_A_MN | UMMA_B_MN;
-    bool ok = true;
+    constexpr uint32_t idesc = umma_idesc(1, fmt, fmt, 256, WG_BK) | UMMA_A_MN | UMMA_B_MN;
     int s = 0; uint32_t ph = 0;
     for (int i = step0; i < step1; ++i) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&full_a[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF10 | s, budget)) ||
-          !__all_sync(0xffffffffu, mbar_wait(&full_b[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF20 | s, budget))) { ok = false; break; }
+      // x^ of the second CTA lies in that CTA's shared memory, and it is that SM's tensor core that reads it there.  The stores are in place when
+      // the arrival leaves the SM: each writer passes them to the async proxy and its warp arrives behind that.  (An arrival with a
+      // release to the cluster also waits for the loads in flight, 1400 clocks of each step: 184 us instead of 106 at M = 65536, N = 2048, K = 512.)
+      if (!__all_sync(0xffffffffu, mbar_wait<true>(&full_a[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF10 | s, budget)) ||
+          !__all_sync(0xffffffffu, mbar_wait<true>(&full_b[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF20 | s, budget))) break;
+      const int in_seg = (i - step0) % WG_SEG;
+      if (in_seg == 0 && i != step0 &&
+          !__all_sync(0xffffffffu, mbar_wait<true>(acc_empty, ((i - step0) / WG_SEG - 1) & 1, abort_flag, ST_TIMEOUT_MMA, 0xF60, budget))) break;
       tc_fence_after();
-      const uint32_t st = smem_u32(smem + s * WG_STAGE);
-      const uint64_t a_desc = umma_smem_desc_mn<128>(st, WG_CHUNK), b_desc = umma_smem_desc_mn<128>(st + WG_A_BYTES, WG_CHUNK);
+      const uint32_t st = smem_u32(smem + s * L::STAGE);
+      const uint64_t a_desc = umma_smem_desc_mn<128>(st, WG_CHUNK), b_desc = umma_smem_desc_mn<128>(st + L::A_BYTES, WG_CHUNK);
       constexpr uint64_t step = (16 * 128) >> 4;           // K = 16: 16 rows of 128 bytes
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        umma_f16_elect(tmem_base, a_desc + step * k, b_desc + step * k, idesc, i != step0 || k != 0);
-        if (two) umma_f16_elect(tmem_base + 256, a_desc + (2 * WG_CHUNK >> 4) + step * k, b_desc + step * k, idesc, i != step0 || k != 0);
+#pragma unroll
+        for (int j = 0; j < ACC; ++j)
+          umma_f16_pair_elect(tmem_base + 256 * j, a_desc + (j * 2 * WG_CHUNK >> 4) + step * k, b_desc + step * k, idesc, in_seg != 0 || k != 0);
       }
-      umma_commit_elect(&empty[s]);
-      if (++s == WG_STAGES) { s = 0; ph ^= 1; }
+      umma_commit_pair_both_elect(&empty[s]);
+      if (in_seg == WG_SEG - 1 || i + 1 == step1) umma_commit_pair_both_elect(acc_full);
+      if (++s == STAGES) { s = 0; ph ^= 1; }
     }
-    if (ok) umma_commit_elect(acc_full);
   } else if (warp >= WG_FRONT) {
-    // Thread: 16 columns of x^ (two 16-byte pieces of a row of the tile), rows r, r + 16, ... of the step.
-    const int tid = threadIdx.x - 32 * WG_FRONT, c = tid & 15, r = tid >> 4;
-    const int k = k0 + 16 * c;
+    // Thread: 16 columns of x^ (two 16-byte pieces of a row of the tile), rows r and r + 32 of the step, loaded WG_AHEAD steps ahead (a step is
+    // shorter than a read of HBM).
+    const int tid = threadIdx.x - 32 * WG_FRONT, c = tid & 7, r = tid >> 3;
+    const int k = k0 + 128 * rank + 16 * c;
     const int have = p.K - k;                              // columns left from k on
-    const uint8_t* qk = p.q + k;
-    const float* sk = p.s + (k < p.K ? (k >> 7) : 0);
-    uint4 raw[4];
-    float sc[4];
-    auto fetch = [&](int i) {
+    const long long dq = 32 * p.ldq, ds = 32 * p.lds;      // (to the thread's other row)
+    const uint8_t* qp = p.q + ((long long)step0 * WG_BM + r) * p.ldq + (have > 0 ? k : 0);
+    const float* sp = p.s + ((long long)step0 * WG_BM + r) * p.lds + (have > 0 ? k >> 7 : 0);
+    uint4 raws[WG_AHEAD][2];
+    float scs[WG_AHEAD][2];
+    auto fetch = [&](int i, uint4 (&raw)[2], float (&sc)[2]) {
+      raw[0] = raw[1] = make_uint4(0u, 0u, 0u, 0u);
+      sc[0] = sc[1] = 0.f;
+      if (i < step1 && have > 0) {
+        // Whole 16-byte pieces: a row's stride holds them (columns behind K end in columns of dW that are not written), only the last row may end
+        // before.
+        const long long left = p.M - ((long long)i * WG_BM + r);     // rows from the thread's first on
+        if ((long long)(i + 1) * WG_BM < p.M) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const long long m = (long long)i * WG_BM + r + 16 * j;
-        raw[j] = make_uint4(0u, 0u, 0u, 0u);
-        sc[j] = 0.f;
-        if (i < step1 && m < p.M && have > 0) {
-          sc[j] = sk[m * p.lds];
-          if (have >= 16) raw[j] = *reinterpret_cast<const uint4*>(qk + m * p.ldq);
-          else {
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int b = 0; b < 15; ++b)
-              if (b < have) w[b >> 2] |= (uint32_t)qk[m * p.ldq + b] << (8 * (b & 3));
-            raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-    };
-    fetch(step0);
-    bool ok = true;
-    int s = 0; uint32_t ph = 0;
-    for (int i = step0; i < step1; ++i) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF30 | s, budget))) { ok = false; break; }
-      uint8_t* tile_b = smem + s * WG_STAGE + WG_A_BYTES + (c >> 2) * WG_CHUNK;
-      const int swap = (c >> 2) & 1;                       // half of the lanes store their second piece first: no bank conflicts
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint4 lo, hi;
-        restore16<T>(raw[j], sc[j], lo, hi);
-        const int row = r + 16 * j, pc = 2 * (c & 3);
-        uint8_t* line = tile_b + row * 128;
-        *reinterpret_cast<uint4*>(line + (((pc + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(line + (((pc + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
-      }
-      fetch(i + 1);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full_b[s]);
-      if (++s == WG_STAGES) { s = 0; ph ^= 1; }
-    }
-    // dW: lane quarter (rows of 32 columns of dY), one accumulator per four warps
-    const int q = warp & 3, half = (warp - WG_FRONT) >> 2;
-    const int n = n0 + 128 * half + 32 * q + lane;
-    const bool any = step1 > step0;                        // (a batch of no rows: all sums are zero)
-    if (ok) ok = !any || __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF40, budget));
-    if (ok && (half == 0 || two)) {
-      tc_fence_after();
-      const uint32_t t = tmem_base + 256 * half + ((uint32_t)(q * 32) << 16);
-      float* o = p.out + part * p.part_stride + (long long)n * p.ldo;
-      const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * 4) | (uintptr_t)(p.part_stride * 4)) & 31) == 0;
-      for (int c0 = 0; c0 < WG_BK && k0 + c0 < p.K; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t + c0, v);
-        tmem_ld_wait(v);
-        if (n >= p.N) continue;
-        float* oc = o + k0 + c0;
-        if (wide && k0 + c0 + 32 <= p.K) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint4 x = make_uint4(v[8 * b], v[8 * b + 1], v[8 * b + 2], v[8 * b + 3]), y = make_uint4(v[8 * b + 4], v[8 * b + 5], v[8 * b + 6], v[8 * b + 7]);
-            if (p.accumulate) {
-              uint4 ox, oy;
-              ldg_v8(oc + 8 * b, ox, oy);
-              x = make_uint4(__float_as_uint(__uint_as_float(x.x) + __uint_as_float(ox.x)), __float_as_uint(__uint_as_float(x.y) + __uint_as_float(ox.y)),
-                             __float_as_uint(__uint_as_float(x.z) + __uint_as_float(ox.z)), __float_as_uint(__uint_as_float(x.w) + __uint_as_float(ox.w)));
-              y = make_uint4(__float_as_uint(__uint_as_float(y.x) + __uint_as_float(oy.x)), __float_as_uint(__uint_as_float(y.y) + __uint_as_float(oy.y)),
-                             __float_as_uint(__uint_as_float(y.z) + __uint_as_float(oy.z)), __float_as_uint(__uint_as_float(y.w) + __uint_as_float(oy.w)));
-            }
-            stg_v8(oc + 8 * b, x, y);
+          for (int j = 0; j < 2; ++j) {
+            raw[j] = *reinterpret_cast<const uint4*>(qp + j * dq);
+            sc[j] = sp[j * ds];
           }
         } else {
 #pragma unroll
-          for (int b = 0; b < 32; ++b)
-            if (k0 + c0 + b < p.K) oc[b] = p.accumulate ? oc[b] + __uint_as_float(v[b]) : __uint_as_float(v[b]);
+          for (int j = 0; j < 2; ++j) {
+            if (left <= 32 * j) continue;
+            sc[j] = sp[j * ds];
+            if (left > 32 * j + 1 || have >= 16) {
+              raw[j] = *reinterpret_cast<const uint4*>(qp + j * dq);
+            } else {
+              uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+              for (int b = 0; b < 15; ++b)
+                if (b < have) w[b >> 2] |= (uint32_t)qp[j * dq + b] << (8 * (b & 3));
+              raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
         }
       }
+      qp += 2 * dq;
+      sp += 2 * ds;
+    };
+#pragma unroll
+    for (int a = 0; a < WG_AHEAD; ++a) fetch(step0 + a, raws[a], scs[a]);
+    const uint32_t arrive_b = mapa_shared(smem_u32(full_b), 0);
+    const int swap = (c >> 2) & 1, pc = 2 * (c & 3);       // half of the lanes store their second piece first: no bank conflicts
+    bool ok = true;
+    // Segment `seg` of the sums to dW.  Warp: lane quarter; of two accumulators one per four warps, of one its column halves.
+    auto drain = [&](int seg) {
+      const int q = warp & 3, half = (warp - WG_FRONT) >> 2;
+      const int n = n0 + (ACC == 2 ? 256 * half : 0) + 32 * q + lane;
+      constexpr int COLS = ACC == 2 ? WG_BK : WG_BK / 2;
+      const int cb = ACC == 2 ? 0 : half * COLS;           // first column of the warp
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, seg & 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF40, budget))) { ok = false; return; }
+      tc_fence_after();
+      const uint32_t t = tmem_base + (ACC == 2 ? 256 * half : cb) + ((uint32_t)(q * 32) << 16);
+      float* o = p.out + part * p.part_stride + (long long)n * p.ldo + k0 + cb;
+      const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * 4) | (uintptr_t)(p.part_stride * 4)) & 31) == 0;
+      const bool add = p.accumulate || seg > 0;
+      for (int c0 = 0; c0 < COLS && k0 + cb + c0 < p.K; c0 += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(t + c0, v);
+        tmem_ld_wait(v);
+        float* oc = o + c0;
+        if (n < p.N && wide && k0 + cb + c0 + 32 <= p.K) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint4 x = make_uint4(v[8 * b], v[8 * b + 1], v[8 * b + 2], v[8 * b + 3]), y = make_uint4(v[8 * b + 4], v[8 * b + 5], v[8 * b + 6], v[8 * b + 7]);
+            if (add) {
+              uint4 ox, oy;
+              ldg_v8(oc + 8 * b, ox, oy);
+              x = add4(x, ox);
+              y = add4(y, oy);
+            }
+            stg_v8(oc + 8 * b, x, y);
+          }
+        } else if (n < p.N) {
+#pragma unroll
+          for (int b = 0; b < 32; ++b)
+            if (k0 + cb + c0 + b < p.K) oc[b] = add ? oc[b] + __uint_as_float(v[b]) : __uint_as_float(v[b]);
+        }
+      }
+    };
+    const uint32_t drained = mapa_shared(smem_u32(acc_empty), 0);
+    static_assert(WG_SEG % WG_AHEAD == 0, "a segment is whole rounds of the loop below");
+    int s = 0; uint32_t ph = 0;
+    for (int i0 = step0; ok && i0 < step1; i0 += WG_AHEAD) {
+      if (i0 != step0 && (i0 - step0) % WG_SEG == 0) {
+        drain((i0 - step0) / WG_SEG - 1);
+        if (!ok) break;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(drained);
+      }
+#pragma unroll
+      for (int a = 0; a < WG_AHEAD; ++a) {
+        const int i = i0 + a;
+        if (i >= step1) break;
+        uint4 lo[2], hi[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) restore16<T>(raws[a][j], scs[a][j], lo[j], hi[j]);
+        fetch(i + WG_AHEAD, raws[a], scs[a]);
+        ok = __all_sync(0xffffffffu, mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF30 | s, budget));
+        if (!ok) break;
+        uint8_t* tile_b = smem + s * L::STAGE + L::A_BYTES + (c >> 2) * WG_CHUNK;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = r + 32 * j;
+          uint8_t* line = tile_b + row * 128;
+          *reinterpret_cast<uint4*>(line + (((pc + swap) ^ (row & 7)) << 4)) = swap ? hi[j] : lo[j];
+          *reinterpret_cast<uint4*>(line + (((pc + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo[j] : hi[j];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(arrive_b + 8 * s);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
     }
+    if (ok) drain((step1 - step0 - 1) / WG_SEG);
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
+  cluster_sync_all();                                      // neither CTA leaves while the other may still arrive at its barriers or its MMAs read here
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem_base, 256 * ACC); }
 }
 
 // dW = (dW +) the parts' sums, in order.
@@ -248,28 +308,53 @@ __global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long par
     }
 }
 
-// Parts the batch is cut into: what fills the SMs with tiles, at least four steps each.  A function of the sizes alone: a workspace
-// asked for before a device is chosen fits, and the sums have the same order everywhere.
-constexpr int WG_FILL = 148;
-static void wgrad_plan(long long M, int N, int K, int& tiles, int& steps, int& parts, long long& ld, long long& part_stride) {
+// Accumulators per CTA, tiles, and the parts the batch is cut into: what fills the SMs with pairs, at least four steps each.  Two accumulators use
+// the restored elements twice, but take half as many pairs for the same tiles and longer to write (us, K = 512, one / two accumulators: N = 2048 M = 333
+// 10.1 / 13.9, 3000 18.8 / 22.5, 9001 30.0 / 29.4, 65536 137 / 104; N = 512 M = 9001 16.8 / 22.5, 65536 43.6 / 42.1): two from 14 steps a part.  A function of the
+// sizes alone: a workspace asked for before a device is chosen fits, and the sums have the same order everywhere.
+constexpr int WG_FILL = 74;
+static void wgrad_plan(long long M, int N, int K, int& acc, int& tiles, int& steps, int& parts, long long& ld, long long& part_stride) {
   const int kt = (K + WG_BK - 1) / WG_BK;
-  tiles = (N + WG_BN - 1) / WG_BN * kt;
   steps = (int)((M + WG_BM - 1) / WG_BM);
-  parts = WG_FILL / tiles;
-  if (parts > steps / 4) parts = steps / 4;
-  if (parts < 1) parts = 1;
+  for (acc = N > 256 ? 2 : 1; ; acc = 1) {
+    tiles = (N + 256 * acc - 1) / (256 * acc) * kt;
+    parts = WG_FILL / tiles;
+    if (parts > steps / 4) parts = steps / 4;
+    if (parts < 1) parts = 1;
+    if (acc == 1 || steps >= 14 * parts) break;
+  }
   ld = ((long long)K + 7) / 8 * 8;
   part_stride = ld * N;
 }
 static bool wgrad_shape_ok(long long M, int N, int K) {
   return M >= 0 && M <= 0x7fffff00ll && N > 0 && K > 0 && N <= (1 << 24) && K <= (1 << 24) &&
-         (long long)((N + WG_BN - 1) / WG_BN) * ((K + WG_BK - 1) / WG_BK) <= (1 << 24);
+         (long long)((N + 255) / 256) * ((K + WG_BK - 1) / WG_BK) <= (1 << 24);
 }
 int64_t wgrad_workspace_bytes(long long M, int N, int K) {
   if (!wgrad_shape_ok(M, N, K)) return 0;
-  int tiles, steps, parts; long long ld, stride;
-  wgrad_plan(M, N, K, tiles, steps, parts, ld, stride);
+  int acc, tiles, steps, parts; long long ld, stride;
+  wgrad_plan(M, N, K, acc, tiles, steps, parts, ld, stride);
   return parts > 1 ? 4 * stride * parts : 0;
+}
+
+template <typename T, int ACC>
+static cudaError_t launch_wg(const CUtensorMap& tm, const WgParams& p, int dev, unsigned grid, cudaStream_t st) {
+  static std::atomic<int> attr_done[64];
+  auto k = wgrad_kernel<T, ACC>;
+  if (!attr_done[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, WgSmem<ACC>::BYTES);
+    if (e != cudaSuccess) return e;
+    attr_done[dev].store(1, std::memory_order_release);
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(WG_THREADS); cfg.dynamicSmemBytes = WgSmem<ACC>::BYTES; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k, tm, p);
 }
 
 int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, long long ldq, const float* s, long long lds, float* dw, long long lddw,
@@ -286,20 +371,14 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
   const int32_t rc = ensure_device();
   if (rc != GSB200_OK) return rc;
   WgParams p{};
+  int acc;
   long long ld, stride;
-  wgrad_plan(M, N, K, p.tiles, p.steps, p.parts, ld, stride);
+  wgrad_plan(M, N, K, acc, p.tiles, p.steps, p.parts, ld, stride);
   const long long need = wgrad_workspace_bytes(M, N, K);
   if (need > 0 && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 31))) return GSB200_ERR_BAD_ARG;
-  static std::atomic<int> attr_done[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return GSB200_ERR_DEVICE;
-  if (!attr_done[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(wgrad_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, WG_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(wgrad_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, WG_BYTES);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(weight gradient)");
-    attr_done[dev].store(1, std::memory_order_release);
-  }
   CUtensorMap tm;
   if (!tmap_2d(&tm, dt == GSB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, (uint64_t)M, (uint64_t)N,
                (uint64_t)lddy, 64, WG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
@@ -307,10 +386,11 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
   const bool cut = p.parts > 1;
   p.out = cut ? static_cast<float*>(ws) : dw; p.ldo = cut ? ld : lddw; p.part_stride = cut ? stride : 0;
   p.accumulate = cut ? 0 : accumulate;
-  const long long grid = (long long)p.tiles * p.parts;
+  const long long grid = 2ll * p.tiles * p.parts;
   if (grid > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
-  cudaError_t e = dt == GSB200_F16 ? launch_dependent(wgrad_kernel<__half>, (unsigned)grid, WG_THREADS, (size_t)WG_BYTES, st, tm, p)
-                                   : launch_dependent(wgrad_kernel<__nv_bfloat16>, (unsigned)grid, WG_THREADS, (size_t)WG_BYTES, st, tm, p);
+  const bool f16 = dt == GSB200_F16;
+  cudaError_t e = acc == 2 ? (f16 ? launch_wg<__half, 2>(tm, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 2>(tm, p, dev, (unsigned)grid, st))
+                           : (f16 ? launch_wg<__half, 1>(tm, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 1>(tm, p, dev, (unsigned)grid, st));
   if (e == cudaSuccess && cut) {
     const long long n4 = (long long)N * ((K + 3) / 4);
     e = launch_dependent(wgrad_reduce_kernel, (unsigned)((n4 + 255) / 256), 256, 0, st, static_cast<const float*>(ws), ld, stride, p.parts, dw, lddw, N, K, accumulate);

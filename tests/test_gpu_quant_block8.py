@@ -214,7 +214,7 @@ def test_gemm_what_lies_behind_the_operands_rows_does_not_matter():
 # ---- weight gradient -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 128), (1, 1, 1), (63, 130, 127), (64, 256, 256), (65, 129, 257), (300, 1000, 520), (2000, 512, 100), (5000, 264, 512),
-                                   (9001, 72, 1001)])
+                                   (9001, 72, 1001), (33000, 264, 200), (40001, 40, 136)])
 def test_wgrad(m, n, k, dt):
     g = need_lib()
     gen = torch.Generator().manual_seed(m + n + k)
