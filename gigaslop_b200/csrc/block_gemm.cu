@@ -9,17 +9,23 @@
 // tensor-memory stage of its own (four MMAs of K = 32 that start from zero), and the epilogue warps add it, times its scale, to fp32 sums
 // in registers: one fused multiply-add per element and K block, since a thread holds one row and 128 columns that share a B scale.
 //
-// Large form: CTA pairs (cta_group::2), tile 256 rows x 256 columns, 128 x 256 per CTA, two tensor-memory stages of 256 columns.
+// Four forms: up to four rows on plain fp32 (block_gemv_kernel), few tiles of 128 rows x 32 to 128 columns (block_gemm_small_kernel), and CTA pairs
+// with tiles of 256 or 128 columns (block_gemm_kernel), which this is about:
+// Tile 256 rows x 256 columns, 128 x 256 per CTA (cta_group::2), two tensor-memory stages of 256 columns (or four of 128).
 //   warp 0      TMA producer (one lane); a CTA loads its 128 rows of A and half of the tile's B, 32 KiB per K block
 //   warp 1      MMA issue (first CTA of the pair; converged, one elected lane)
-//   warps 2, 3  products of the scales, two K blocks ahead, through shared memory
+//   warps 2, 3  products of the scales, loaded four K blocks ahead, through shared memory
 //   warps 4..11 epilogue: lane quarter e % 4, column half e / 4
 // What bounds it is the round trip of a stage, two of which are all that tensor memory holds: MMAs (512 clocks and about 230 until the last
 // one shows), the epilogue's wake-up, four reads of 32 columns (300), the return to the MMA warp (230): about 1700 clocks for two
 // K blocks, 850 each where the MMAs alone take 512.  Everything that can leave that chain has left it: the scales (their address arithmetic,
 // loads and products), the wait for the operands (before that for the stage), the multiply-adds of a chunk (behind the read of the next one,
 // the last ones behind the release).  us, M = 65536, N = 1536, K = 512 / N = 512, K = 2048: single CTAs with 256 columns that load their own scales
-// 91 / 80; pairs 95 / 80; scales through shared memory 78 / 76; two staging boxes per warp instead of one 72 / 74.
+// 91 / 80; pairs 95 / 80; scales through shared memory 78 / 76; two staging boxes per warp instead of one 72 / 74, filled before one fence 70 / 72.
+// Tried and dropped: results straight from registers in 32-byte sectors (92 / 78).
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
 #include <atomic>
 
 #include "capi_internal.h"
@@ -27,28 +33,34 @@
 
 namespace gsb {
 
-constexpr int BG_BM = 128, BG_BN = 256, BG_BK = 128;
+constexpr int BG_BM = 128, BG_BK = 128;
 constexpr int BG_EPI_WARPS = 8, BG_FRONT_WARPS = 4;
 constexpr int BG_FRONT_REGS = 56, BG_EPI_REGS = 224;
 constexpr int BG_THREADS = 32 * (BG_EPI_WARPS + BG_FRONT_WARPS);
 constexpr int BG_A_BYTES = BG_BM * BG_BK;                  // 16 KiB
-constexpr int BG_ACC = 2;                                  // tensor-memory stages
 constexpr int BG_OUT_BUF = 2 * 4096;                       // per epilogue warp: two boxes of 32 rows x 128 bytes
-
-constexpr int BG_SC = 4;                                   // K blocks of scales in shared memory
-
-constexpr int BG_B_BYTES = BG_BN / 2 * BG_BK;              // a CTA of the pair holds half of the tile's columns
-constexpr int BG_STAGE = BG_A_BYTES + BG_B_BYTES;          // 32 KiB
-constexpr int BG_STAGES = 4;
-constexpr int BG_OUT = BG_STAGES * BG_STAGE;
-constexpr int BG_SCALES = BG_OUT + BG_EPI_WARPS * BG_OUT_BUF;             // [BG_SC][2][BG_BM] products of the scales
-constexpr int BG_BAR = BG_SCALES + BG_SC * 2 * BG_BM * 4;
-constexpr int BG_BYTES = BG_BAR + 256 + 1024;
-static_assert(BG_BYTES <= 227 * 1024, "shared memory budget");
+// The large form with tiles of BN columns
+template <int BN>
+struct BgSmem {
+  static constexpr int ACC = 512 / BN;                     // tensor-memory stages
+  static constexpr int STAGE = BG_A_BYTES + BN / 2 * BG_BK;               // a CTA of the pair holds half of the tile's columns: 32 or 24 KiB
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int SC = 2 * ACC;                       // K blocks of scales in shared memory
+  static constexpr int OUT = STAGES * STAGE;
+  static constexpr int SCALES = OUT + BG_EPI_WARPS * BG_OUT_BUF;          // [SC][2][BG_BM] products of the scales
+  static constexpr int BAR = SCALES + SC * 2 * BG_BM * 4;
+  static constexpr int BYTES = BAR + 256 + 1024;
+  static_assert(BYTES <= 227 * 1024 && (2 * STAGES + 2 * ACC) * 8 + 8 <= 256, "shared memory budget");
+};
 
 __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two E4M3 values (the low 16 bits) as fp32
+__device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
 struct BgParams {
@@ -56,24 +68,26 @@ struct BgParams {
   const float* sa; long long ld_sa;
   const float* sb; long long ld_sb_n, ld_sb_k;             // B scale of (column block, K block): sb[cb * ld_sb_n + kb * ld_sb_k]
   void* C; long long ldc; int c_type;
+  int a_rows;                                              // few-tile form: rows of the boxes of A
   int n_tma;                                               // the columns before it leave through TMA boxes, the others element by element
 };
 
 // KN: B is [K, N].  Its stage holds boxes of 128 K rows x 128 columns.
-template <bool KN>
+template <int BN, bool KN>
 __global__ void __launch_bounds__(BG_THREADS, 1)
 block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_c,
                   const BgParams p) {
   extern __shared__ uint8_t bg_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(bg_smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int BN = BG_BN, ACC = BG_ACC, STAGES = BG_STAGES;
+  using L = BgSmem<BN>;
+  constexpr int ACC = L::ACC, STAGES = L::STAGES, SC = L::SC;
   constexpr int CW = BN / 2;                               // columns of an epilogue warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + BG_BAR);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + ACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACC);
-  float* sc_smem = reinterpret_cast<float*>(smem + BG_SCALES);
+  float* sc_smem = reinterpret_cast<float*>(smem + L::SCALES);
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_tiles = p.m_blocks * p.n_blocks;           // (the host keeps this below 2^31)
@@ -98,7 +112,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const unsigned int budget = spin_budget();
 
   if (warp < BG_FRONT_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BG_FRONT_REGS));
+    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BG_FRONT_REGS));
     if (warp == 0) {
       if (lane == 0) {
         bool ok = true;
@@ -107,11 +121,11 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           const int m0 = tile_row(t), n0 = tile_col(t) + rank * (BN / 2);
           for (int kb = 0; kb < p.k_blocks; ++kb) {
             if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE00 | s, budget)) { ok = false; break; }
-            uint8_t* st = smem + s * BG_STAGE;
+            uint8_t* st = smem + s * L::STAGE;
             auto load = [&](void* dst, const CUtensorMap* m, int x, int y) {
               tma_load_2d_pair(dst, m, mapa_shared(smem_u32(&full[s]), 0), x, y);
             };
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * BG_STAGE);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
             load(st, &tm_a, kb * BG_BK, m0);
             if constexpr (KN) load(st + BG_A_BYTES, &tm_b, n0, kb * BG_BK);
             else load(st + BG_A_BYTES, &tm_b, kb * BG_BK, n0);
@@ -128,12 +142,12 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           // (the stage's return last: it is what the MMAs wait for)
           if (!__all_sync(0xffffffffu, mbar_wait<true>(&full[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xE20 | s, budget))) { ok = false; break; }
-          const uint32_t st = smem_u32(smem + s * BG_STAGE);
+          const uint32_t st = smem_u32(smem + s * L::STAGE);
           const uint64_t a_desc = umma_smem_desc_sw128(st);
-          const uint64_t b_desc = KN ? umma_smem_desc_mn<128>(st + BG_A_BYTES, 128 * BG_BK) : umma_smem_desc_sw128(st + BG_A_BYTES);
+          const uint64_t b_desc = KN ? umma_smem_desc_mn<BN / 2>(st + BG_A_BYTES, 0) : umma_smem_desc_sw128(st + BG_A_BYTES);
           if (!__all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE10 | as, budget))) { ok = false; break; }
           tc_fence_after();
-          constexpr uint64_t b_step = KN ? (32 * 128) >> 4 : 2;           // K = 32: 32 rows of 128 bytes, or 32 bytes of a row
+          constexpr uint64_t b_step = KN ? (32 * (BN / 2)) >> 4 : 2;      // K = 32: 32 rows of BN / 2 bytes, or 32 bytes of a row
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_f8_pair_elect(tmem_base + as * BN, a_desc + 2 * k, b_desc + b_step * k, idesc, k != 0);
           umma_commit_pair_both_elect(&acc_full[as]);
@@ -143,12 +157,13 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
       }
     } else if (warp >= 2) {
-      // The products of the scales, ahead of the MMAs: two rows and both column halves per lane, loaded two K blocks ahead.  A K
+      // The products of the scales, ahead of the MMAs: two rows and both column halves per lane, loaded ahead.  A K
       // block's arrival completes acc_full together with the MMAs' (the one wait of the epilogue covers both), and must follow the
-      // barrier's previous phase.  By then the MMAs two K blocks back were allowed to start, so the epilogue is done with the K block four
-      // back, whose place this one takes.
+      // barrier's previous phase, ACC K blocks back.  By then those MMAs were allowed to start, so the epilogue is done with the K block
+      // 2 ACC back, whose place this one takes.
       const int r = (warp - 2) * 64 + lane;
-      float a0[2], a1[2], b0[2], b1[2];
+      constexpr int FAR = 4;                                 // K blocks that are loaded ahead
+      float a0[FAR], a1[FAR], b0[FAR], b1[FAR];
       int ft = unit, fkb = 0;                                // what is fetched next
       auto fetch_next = [&](int j) {
         if (ft < num_tiles) {
@@ -157,36 +172,39 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           a1[j] = ldg_f_here(p.sa + (long long)(m + 32 < p.M ? m + 32 : p.M - 1) * p.ld_sa + fkb);
           const float* sb = p.sb + (long long)fkb * p.ld_sb_k + (long long)(n >> 7) * p.ld_sb_n;
           b0[j] = ldg_f_here(sb);
-          b1[j] = n + 128 < p.N ? ldg_f_here(sb + p.ld_sb_n) : 0.f;
+          b1[j] = BN == 128 ? b0[j] : n + 128 < p.N ? ldg_f_here(sb + p.ld_sb_n) : 0.f;
         }
         if (++fkb == p.k_blocks) { fkb = 0; ft += units; }
       };
-      a0[0] = a0[1] = a1[0] = a1[1] = b0[0] = b0[1] = b1[0] = b1[1] = 0.f;
-      fetch_next(0);
-      fetch_next(1);
+#pragma unroll
+      for (int j = 0; j < FAR; ++j) { a0[j] = a1[j] = b0[j] = b1[j] = 0.f; fetch_next(j); }
       bool ok = true;
       uint32_t i = 0;
       auto put = [&](int j) {
-        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait<true>(&acc_full[j], ((i - 2) >> 1) & 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE40 | j, budget))) { ok = false; return; }
-        float* d = sc_smem + (i & (BG_SC - 1)) * 2 * BG_BM + r;
+        const uint32_t as = i % ACC;
+        if (i >= ACC && !__all_sync(0xffffffffu, mbar_wait<true>(&acc_full[as], (i / ACC - 1) & 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE40 | as, budget))) { ok = false; return; }
+        float* d = sc_smem + i % SC * 2 * BG_BM + r;
         d[0] = a0[j] * b0[j]; d[32] = a1[j] * b0[j]; d[BG_BM] = a0[j] * b1[j]; d[BG_BM + 32] = a1[j] * b1[j];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_full[j]);
+        if (lane == 0) mbar_arrive(&acc_full[as]);
         fetch_next(j);
         ++i;
       };
-      for (int t = unit; ok && t < num_tiles; t += units)
-        for (int kb = 0; ok && kb < p.k_blocks; ++kb) { if (i & 1) put(1); else put(0); }
+      const uint32_t all = (uint32_t)((num_tiles - unit + units - 1) / units) * (uint32_t)p.k_blocks;      // (unit < num_tiles; bounded by the host)
+      while (ok && i < all) {
+#pragma unroll
+        for (int j = 0; j < FAR; ++j)
+          if (ok && i < all) put(j);
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BG_EPI_REGS));
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BG_EPI_REGS));      // (128 sums; with 64 the even share is enough)
     const int e = warp - BG_FRONT_WARPS, q = warp & 3, half = e >> 2;
     const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + half * CW;
     bool ok = true;
     const float* const sc_lane = sc_smem + half * BG_BM + q * 32 + lane;
     const uint32_t release_addr = mapa_shared(smem_u32(&acc_empty[0]), 0);
-    uint32_t it = 0;                                         // K blocks so far: stage it % 2, phase it / 2 % 2
-    static_assert(ACC == 2, "");
+    uint32_t it = 0;                                         // K blocks so far: stage it % ACC, phase it / ACC % 2
     for (int t = unit; ok && t < num_tiles; t += units) {
       const int m0 = tile_row(t) + q * 32, n0 = tile_col(t) + half * CW;
       const int row = m0 + lane;
@@ -197,13 +215,13 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       // A chain of 32-column chunks: while one is added, the next is on its way from tensor memory, across K blocks too if the next
       // stage is there already; a stage goes back as soon as its last chunk is in registers.
       uint32_t v[2][32];
-      auto stage_there = [&]() { return __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[it & 1], (it >> 1) & 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xE30, budget)); };
+      auto stage_there = [&]() { return __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[it % ACC], (it / ACC) & 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xE30, budget)); };
       ok = stage_there();
       if (!ok) break;
       tc_fence_after();
-      tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
+      tmem_ld_32x32b_x32(t_lane + it % ACC * BN, v[0]);
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        const float sc = sc_lane[(it & (BG_SC - 1)) * 2 * BG_BM];
+        const float sc = sc_lane[it % SC * 2 * BG_BM];
         const bool more = kb + 1 < p.k_blocks;
         const float2 s2 = pk2(sc, sc);
         bool there = false;
@@ -211,15 +229,15 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         for (int c = 0; c < CW / 32; ++c) {
           tmem_ld_wait(v[c & 1]);
           if (c + 1 < CW / 32) {
-            tmem_ld_32x32b_x32(t_lane + (it & 1) * BN + 32 * (c + 1), v[(c + 1) & 1]);
+            tmem_ld_32x32b_x32(t_lane + it % ACC * BN + 32 * (c + 1), v[(c + 1) & 1]);
           } else {
             tc_fence_before();
-            if (lane == 0) mbar_arrive_remote_relaxed(release_addr + 8 * (it & 1));
+            if (lane == 0) mbar_arrive_remote_relaxed(release_addr + 8 * (it % ACC));
             ++it;
-            there = more && __all_sync(0xffffffffu, mbar_test_wait(&acc_full[it & 1], (it >> 1) & 1));
+            there = more && __all_sync(0xffffffffu, mbar_test_wait(&acc_full[it % ACC], (it / ACC) & 1));
             if (there) {
               tc_fence_after();
-              tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
+              tmem_ld_32x32b_x32(t_lane + it % ACC * BN, v[0]);
             }
           }
 #pragma unroll
@@ -233,57 +251,59 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           ok = stage_there();
           if (!ok) break;
           tc_fence_after();
-          tmem_ld_32x32b_x32(t_lane + (it & 1) * BN, v[0]);
+          tmem_ld_32x32b_x32(t_lane + it % ACC * BN, v[0]);
         }
       }
       if (!ok || !live) continue;
-      // 32 columns at a time.  Boxes of 32 rows x 128 bytes (32 columns of fp32, 64 of 16 bits) in the 128-byte swizzle.
-      const bool f32 = p.c_type == GSB200_F32;
+      // Boxes of 32 rows x 128 bytes (32 columns of fp32, 64 of 16 bits) in the 128-byte swizzle, two at a time.
+      uint8_t* const out_buf = smem + L::OUT + e * BG_OUT_BUF;
+      uint8_t* const line = out_buf + lane * 128;
+      const int wide = p.c_type == GSB200_F32 ? 32 : 64;       // columns of a box
+      auto boxes = [&](auto pack8, auto most, int first, int n_boxes) {        // pack8(bx, pc): 16-byte piece pc of a row of box bx
+        if (lane == 0) tma_store_wait_read<0>();             // the previous boxes have left the buffer
+        __syncwarp();
 #pragma unroll
-      for (int b = 0; b < CW / 32; ++b) {
-        const int n = n0 + 32 * b, box = f32 ? n : n0 + 32 * (b & ~1);
-        if (n >= p.N) break;
-        if (box >= p.n_tma) {
-          if (row < p.M) {
+        for (int bx = 0; bx < decltype(most)::value; ++bx)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (n + i >= p.N) continue;
-              const long long o = (long long)row * p.ldc + n + i;
-              const float v = acc[32 * b + i];
-              if (f32) static_cast<float*>(p.C)[o] = v;
-              else if (p.c_type == GSB200_F16) static_cast<__half*>(p.C)[o] = __float2half_rn(v);
-              else static_cast<__nv_bfloat16*>(p.C)[o] = __float2bfloat16_rn(v);
-            }
+          for (int pc = 0; pc < 8; ++pc) *reinterpret_cast<uint4*>(line + bx * (BG_OUT_BUF / 2) + ((pc ^ (lane & 7)) << 4)) = pack8(bx, pc);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          for (int bx = 0; bx < n_boxes; ++bx) tma_store_2d(&tm_c, out_buf + bx * (BG_OUT_BUF / 2), first + bx * wide, m0);
+          tma_store_commit();
+        }
+      };
+      const int tma_cols = p.n_tma - n0;                       // columns of this warp that leave through boxes
+      if (tma_cols > 0) {
+        if (p.c_type == GSB200_F32) {
+#pragma unroll
+          for (int c0 = 0; c0 < CW; c0 += 64) {
+            if (c0 >= tma_cols) break;
+            boxes([&](int bx, int pc) {
+              const float* a = acc + c0 + 32 * bx + 4 * pc;
+              return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+            }, std::integral_constant<int, 2>{}, n0 + c0, tma_cols - c0 > 32 ? 2 : 1);
           }
-          continue;
-        }
-        uint8_t* const out_buf = smem + BG_OUT + e * BG_OUT_BUF + (f32 ? b & 1 : b >> 1) * (BG_OUT_BUF / 2);
-        if (f32 || (b & 1) == 0) {
-          if (lane == 0) tma_store_wait_read<1>();           // the box before the previous one has left the buffer
-          __syncwarp();
-        }
-        if (f32) {
-#pragma unroll
-          for (int pc = 0; pc < 8; ++pc)
-            *reinterpret_cast<float4*>(out_buf + lane * 128 + ((pc ^ (lane & 7)) << 4)) =
-                make_float4(acc[32 * b + 4 * pc], acc[32 * b + 4 * pc + 1], acc[32 * b + 4 * pc + 2], acc[32 * b + 4 * pc + 3]);
+        } else if (p.c_type == GSB200_F16) {
+          boxes([&](int bx, int pc) {
+            const float* a = acc + 64 * bx + 8 * pc;
+            return make_uint4(pack_half2(a[0], a[1]), pack_half2(a[2], a[3]), pack_half2(a[4], a[5]), pack_half2(a[6], a[7]));
+          }, std::integral_constant<int, CW / 64>{}, n0, CW > 64 && tma_cols > 64 ? 2 : 1);
         } else {
-#pragma unroll
-          for (int pc = 0; pc < 4; ++pc) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float lo = acc[32 * b + 8 * pc + 2 * j], hi = acc[32 * b + 8 * pc + 2 * j + 1];
-              if (p.c_type == GSB200_F16) w[j] = pack_half2(lo, hi);
-              else w[j] = pack_bf2(lo, hi);
-            }
-            *reinterpret_cast<uint4*>(out_buf + lane * 128 + (((4 * (b & 1) + pc) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          boxes([&](int bx, int pc) {
+            const float* a = acc + 64 * bx + 8 * pc;
+            return make_uint4(pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3]), pack_bf2(a[4], a[5]), pack_bf2(a[6], a[7]));
+          }, std::integral_constant<int, CW / 64>{}, n0, CW > 64 && tma_cols > 64 ? 2 : 1);
         }
-        if (f32 || (b & 1) == 1 || n + 32 >= p.N || b + 1 == CW / 32) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) { tma_store_2d(&tm_c, out_buf, box, m0); tma_store_commit(); }
+      }
+      if (tma_cols < CW && p.n_tma < p.N && row < p.M) {       // what TMA cannot address, element by element
+        const long long o = (long long)row * p.ldc + n0;
+#pragma unroll
+        for (int i = 0; i < CW; ++i) {
+          if (i < tma_cols || n0 + i >= p.N) continue;
+          if (p.c_type == GSB200_F32) static_cast<float*>(p.C)[o + i] = acc[i];
+          else if (p.c_type == GSB200_F16) static_cast<__half*>(p.C)[o + i] = __float2half_rn(acc[i]);
+          else static_cast<__nv_bfloat16*>(p.C)[o + i] = __float2bfloat16_rn(acc[i]);
         }
       }
     }
@@ -297,7 +317,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 
 // ---- few tiles ---------------------------------------------------------------------------------------------------------
 // One tile of 128 rows x BN columns per CTA.  With few rows the time is a chain of latencies: the narrow tile spreads the weight over the SMs,
-// and a K block takes BN tensor-memory columns, so that up to 512 / BN of them are multiplied before the first has been added.
+// a K block takes BN tensor-memory columns, so that up to 512 / BN of them are multiplied before the first has been added, and of a single
+// row block only the rows that are there are loaded.  N = 2048, K = 512: 64 rows 3.1 us, 333 3.7, 1000 4.7 (single CTAs with 256 columns 6.2, 6.6, 6.8).
 //   warp 0 TMA producer, warp 1 MMA issue, warps 2..9 epilogue (lane quarter w % 4, column half), results straight from registers
 constexpr int BS_THREADS = 32 * 10;
 template <int BN>
@@ -347,9 +368,10 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
       bool ok = true;
       int s = 0; uint32_t ph = 0;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        if (!mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE50 | s, budget)) { ok = false; break; }
+        if (kb >= STAGES && !mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE50 | s, budget)) { ok = false; break; }
         uint8_t* st = smem + s * L::STAGE;
-        mbar_arrive_expect_tx(&full[s], L::STAGE);
+        // (of a single row block only the rows that are there: what the others hold stays in rows that are not written)
+        mbar_arrive_expect_tx(&full[s], p.a_rows * BG_BK + BN * BG_BK);
         tma_load_2d(st, &tm_a, &full[s], kb * BG_BK, m0);
         if constexpr (KN) tma_load_2d(st + BG_A_BYTES, &tm_b, &full[s], n0, kb * BG_BK);
         else tma_load_2d(st + BG_A_BYTES, &tm_b, &full[s], kb * BG_BK, n0);
@@ -362,7 +384,7 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     int s = 0, as = 0; uint32_t ph = 0, aph = 0;
     for (int kb = 0; kb < p.k_blocks; ++kb) {
       if (!__all_sync(0xffffffffu, mbar_wait<true>(&full[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xE60 | s, budget))) break;
-      if (!__all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE70 | as, budget))) break;
+      if (kb >= ACC && !__all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[as], aph ^ 1, abort_flag, ST_TIMEOUT_MMA, 0xE70 | as, budget))) break;
       tc_fence_after();
       const uint32_t st = smem_u32(smem + s * L::STAGE);
       const uint64_t a_desc = umma_smem_desc_sw128(st);
@@ -371,7 +393,7 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
 #pragma unroll
       for (int k = 0; k < 4; ++k) umma_f8_elect(tmem_base + as * BN, a_desc + 2 * k, b_desc + b_step * k, idesc, k != 0);
       umma_commit_elect(&acc_full[as]);
-      umma_commit_elect(&empty[s]);
+      if (kb + STAGES < p.k_blocks) umma_commit_elect(&empty[s]);
       if (++s == STAGES) { s = 0; ph ^= 1; }
       if (++as == ACC) { as = 0; aph ^= 1; }
     }
@@ -474,30 +496,120 @@ static cudaError_t launch_bs(const CUtensorMap& ta, const CUtensorMap& tb, const
   return launch_dependent(k, (unsigned)grid, BS_THREADS, (size_t)BsSmem<BN>::BYTES, st, ta, tb, p);
 }
 
+// ---- a few rows -----------------------------------------------------------------------------------------------------------
+// Up to four rows, B [N, K] (a decoder's products): the time is the read of the weight, and a tensor-core tile would spend 0.3 us on each
+// K block of a chain.  A warp owns a column: a lane reads 16 consecutive elements of it per 512, multiplies them in fp32 with A's (as fp32 in shared
+// memory, in the order in which the lanes read them without conflicts), and the 16 products' sum, times the block's scale, goes to the lane's sum;
+// the lanes' are added at the end, in a fixed order.  us, this / the few-tile form: one row N = 2048, K = 512 2.0 / 3.1, N = 512, K = 2048 2.8 / 6.3, N = 4096,
+// K = 4096 6.9 / 11.6; two rows 2.3 / 3.1, 3.5 / 6.3, 10.4 / 11.6; four 3.0 / 3.1, 5.1 / 6.3 and, N = 4096, K = 1024, 6.2 / 4.3 (every CTA lays A out): three
+// and four rows up to a million weights.
+constexpr int GV_WARPS = 8;
+constexpr int GV_MAX = 10240;                              // elements of A in shared memory (rows x K, K rounded up to 512)
+template <int ROWS>
+__global__ void __launch_bounds__(GV_WARPS * 32)
+block_gemv_kernel(const uint8_t* A, long long lda, const uint8_t* B, long long ldb, int K, const BgParams p) {
+  __shared__ float4 a_s[GV_MAX / 4];                       // [K / 512][row][4][lane]: elements 512 i + 16 lane + 4 j ..
+  __shared__ float sc_s[GV_MAX / 128];                     // [row][K block] products of the scales
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_base = blockIdx.x * GV_WARPS, n = n_base + warp;
+  const int rounds = (K + 511) / 512;
+  pdl_wait();
+  pdl_trigger();
+  // the column's first elements are on their way while A is laid out
+  const uint8_t* b = B + (long long)(n < p.N ? n : p.N - 1) * ldb;
+  auto load_b = [&](int i) {
+    const int k = 512 * i + 16 * lane;
+    if (k + 16 <= K) return *reinterpret_cast<const uint4*>(b + k);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 15; ++j)
+      if (k + j < K) w[j >> 2] |= (uint32_t)b[k + j] << (8 * (j & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  uint4 next = load_b(0);
+  for (int i = threadIdx.x; i < ROWS * rounds * 128; i += GV_WARPS * 32) {      // four elements at a time
+    const int l = i & 31, j = (i >> 5) & 3, m = (i >> 7) % ROWS, r = (i >> 7) / ROWS;
+    const int k = 512 * r + 16 * l + 4 * j;
+    uint32_t w = 0u;
+    if (m < p.M && k < K) {
+      const uint8_t* a = A + (long long)m * lda + k;
+      if (k + 4 <= K) w = *reinterpret_cast<const uint32_t*>(a);
+      else {
+#pragma unroll
+        for (int t = 0; t < 3; ++t)
+          if (k + t < K) w |= (uint32_t)a[t] << (8 * t);
+      }
+    }
+    const float2 lo = e4m3x2_f32(w), hi = e4m3x2_f32(w >> 16);
+    a_s[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+  }
+  for (int i = threadIdx.x; i < ROWS * p.k_blocks; i += GV_WARPS * 32) {
+    const int m = i / p.k_blocks, kb = i % p.k_blocks;
+    sc_s[i] = m < p.M ? p.sa[(long long)m * p.ld_sa + kb] * p.sb[(long long)(n_base >> 7) * p.ld_sb_n + kb] : 0.f;
+  }
+  __syncthreads();
+  float sum[ROWS];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) sum[m] = 0.f;
+  for (int r = 0; r < rounds; ++r) {
+    const uint32_t w[4] = {next.x, next.y, next.z, next.w};
+    if (r + 1 < rounds) next = load_b(r + 1);
+    const int kb = 4 * r + (lane >> 3);
+    float2 part[ROWS];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) part[m] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 lo = e4m3x2_f32(w[j]), hi = e4m3x2_f32(w[j] >> 16);
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        const float4 a = a_s[((r * ROWS + m) * 4 + j) * 32 + lane];
+        part[m] = __ffma2_rn(make_float2(a.x, a.y), lo, part[m]);
+        part[m] = __ffma2_rn(make_float2(a.z, a.w), hi, part[m]);
+      }
+    }
+    if (kb < p.k_blocks) {
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) sum[m] = fmaf(part[m].x + part[m].y, sc_s[m * p.k_blocks + kb], sum[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], d);
+    if (lane == 0 && n < p.N && m < p.M) {
+      const long long o = (long long)m * p.ldc + n;
+      if (p.c_type == GSB200_F32) static_cast<float*>(p.C)[o] = sum[m];
+      else if (p.c_type == GSB200_F16) static_cast<__half*>(p.C)[o] = __float2half_rn(sum[m]);
+      else static_cast<__nv_bfloat16*>(p.C)[o] = __float2bfloat16_rn(sum[m]);
+    }
+  }
+}
+
 // Launches `units` pairs; units = 0 asks how many can be resident (0: this form must not be launched here).
-template <bool KN>
+template <int BN, bool KN>
 static cudaError_t launch_bg(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const BgParams& p, int dev, int units, int* capacity,
                              cudaStream_t st) {
   static std::atomic<int> cap[64];
-  auto k = block_gemm_kernel<KN>;
+  auto k = block_gemm_kernel<BN, KN>;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(BG_THREADS); cfg.dynamicSmemBytes = BG_BYTES; cfg.stream = st;
+  cfg.blockDim = dim3(BG_THREADS); cfg.dynamicSmemBytes = BgSmem<BN>::BYTES; cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 2;
   int c = cap[dev].load(std::memory_order_acquire);
   if (c == 0) {
     // the re-split of the registers waits until the block's own pool covers it
     cudaFuncAttributes fa{};
     cudaError_t e = cudaFuncGetAttributes(&fa, k);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BG_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BgSmem<BN>::BYTES);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3((unsigned)(sm_count_physical() / 2 * 2));
     int n = 0;
-    const bool pool = fa.numRegs * BG_THREADS >= 32 * (BG_FRONT_WARPS * BG_FRONT_REGS + BG_EPI_WARPS * BG_EPI_REGS) && fa.numRegs * BG_THREADS <= 65536;
+    const bool pool = BN != 256 || (fa.numRegs * BG_THREADS >= 32 * (BG_FRONT_WARPS * BG_FRONT_REGS + BG_EPI_WARPS * BG_EPI_REGS) && fa.numRegs * BG_THREADS <= 65536);
     c = pool && cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0 ? n : -1;
     (void)cudaGetLastError();
     cap[dev].store(c, std::memory_order_release);
@@ -505,6 +617,12 @@ static cudaError_t launch_bg(const CUtensorMap& ta, const CUtensorMap& tb, const
   if (units == 0) { *capacity = c > 0 ? c : 0; return cudaSuccess; }
   cfg.gridDim = dim3((unsigned)(2 * units));
   return cudaLaunchKernelEx(&cfg, k, ta, tb, tc, p);
+}
+
+static cudaError_t launch_bg_form(int pn, bool kn, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const BgParams& p, int dev, int units,
+                                  int* capacity, cudaStream_t st) {
+  return pn == 256 ? (kn ? launch_bg<256, true>(ta, tb, tc, p, dev, units, capacity, st) : launch_bg<256, false>(ta, tb, tc, p, dev, units, capacity, st))
+                   : (kn ? launch_bg<128, true>(ta, tb, tc, p, dev, units, capacity, st) : launch_bg<128, false>(ta, tb, tc, p, dev, units, capacity, st));
 }
 
 int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb, const float* sb,
@@ -524,22 +642,34 @@ int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return GSB200_ERR_DEVICE;
-  CUtensorMap ta, tb, tc;
+  CUtensorMap ta{}, tb{}, tc{};
   BgParams p{};
   p.M = (int)M; p.N = N; p.k_blocks = kb;
   p.sa = sa; p.ld_sa = ld_sa; p.sb = sb; p.ld_sb_n = kn ? 1 : ld_sb; p.ld_sb_k = kn ? ld_sb : 1;
   p.C = C; p.ldc = ldc; p.c_type = c_type;
+  const long long a_elems = (long long)(K + 511) / 512 * 512 * (M <= 2 ? M : 4);
+  if (!kn && a_elems <= GV_MAX && (M <= 2 || (M <= 4 && (long long)N * K <= (1 << 20)))) {
+    const unsigned g = (unsigned)((N + GV_WARPS - 1) / GV_WARPS);
+    const cudaError_t e = M == 1 ? launch_dependent(block_gemv_kernel<1>, g, GV_WARPS * 32, 0, st, A, lda, B, ldb, K, p)
+                        : M == 2 ? launch_dependent(block_gemv_kernel<2>, g, GV_WARPS * 32, 0, st, A, lda, B, ldb, K, p)
+                                 : launch_dependent(block_gemv_kernel<4>, g, GV_WARPS * 32, 0, st, A, lda, B, ldb, K, p);
+    return cuda_status(e, "block-scaled gemm launch");
+  }
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  if (!tmap_2d(&ta, u8, 1, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BG_BK, BG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   const int sms = sm_count();
   const long long rb = (M + BG_BM - 1) / BG_BM;
   int bn = 0;                                                // the narrowest tile of which all are resident at once; none: pairs
   for (int w = 32; w <= 128 && bn == 0; w *= 2)
     if (rb * ((N + w - 1) / w) <= sms) bn = w;
-  int units = 0;
+  int units = 0, pn = 256;                                   // pairs, and the columns of their tiles
   if (bn == 0) {
+    const long long rb2 = (M + 2 * BG_BM - 1) / (2 * BG_BM);
+    // 128 columns where their rounds are cheaper: a tile takes 0.57 of the time of a 256-column one up to K = 512, 0.69 from there on (us, 256 / 128
+    // columns, M = 65536: K = 512 N = 128 16.0 / 12.9, 640 41.0 / 40.4, 1536 70.6 / 80.2; K = 384, N = 384 25.9 / 23.4; K = 2048, N = 512 71.1 / 98.5)
+    const long long r256 = (rb2 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2 > 0 ? sms / 2 : 1), r128 = (rb2 * nb + sms / 2 - 1) / (sms / 2 > 0 ? sms / 2 : 1);
+    if (r128 * (kb <= 4 ? 60 : 69) < r256 * 100) pn = 128;
     int cap = 0;
-    const cudaError_t e = kn ? launch_bg<true>(ta, ta, ta, p, dev, 0, &cap, st) : launch_bg<false>(ta, ta, ta, p, dev, 0, &cap, st);
+    const cudaError_t e = launch_bg_form(pn, kn, ta, ta, ta, p, dev, 0, &cap, st);
     if (e != cudaSuccess) return cuda_status(e, "block-scaled gemm set-up");
     units = sms / 2 < cap ? sms / 2 : cap;
     if (units == 0) bn = 128;
@@ -548,6 +678,8 @@ int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long
     p.m_blocks = (int)rb; p.n_blocks = (N + bn - 1) / bn;
     const long long tiles = rb * p.n_blocks;
     if (tiles > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
+    p.a_rows = M < BG_BM ? (int)((M + 7) / 8 * 8) : BG_BM;
+    if (!tmap_2d(&ta, u8, 1, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BG_BK, (uint32_t)p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
     const CUtensorMapSwizzle sw = bn == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bn == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
     if (kn ? !tmap_2d(&tb, u8, 1, B, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, (uint32_t)bn, BG_BK, sw)
            : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, (uint32_t)bn, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
@@ -557,21 +689,21 @@ int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long
                                    : (kn ? launch_bs<128, true>(ta, tb, p, dev, g, st) : launch_bs<128, false>(ta, tb, p, dev, g, st));
     return cuda_status(e, "block-scaled gemm launch");
   }
-  p.m_blocks = (int)((M + 2 * BG_BM - 1) / (2 * BG_BM)); p.n_blocks = (N + BG_BN - 1) / BG_BN;
+  p.m_blocks = (int)((M + 2 * BG_BM - 1) / (2 * BG_BM)); p.n_blocks = (N + pn - 1) / pn;
   const long long tiles = (long long)p.m_blocks * p.n_blocks;
   if (tiles > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
+  if (!tmap_2d(&ta, u8, 1, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BG_BK, BG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   // TMA writes whole 16-byte pieces: where a row of C ends inside one, the last box goes element by element
   const bool tma_out = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * esz) % 16 == 0;
   p.n_tma = !tma_out ? 0 : (N * esz) % 16 == 0 ? N : N / (128 / esz) * (128 / esz);
   const CUtensorMapDataType ct = c_type == GSB200_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                : c_type == GSB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (kn ? !tmap_2d(&tb, u8, 1, B, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, 128, BG_BK, CU_TENSOR_MAP_SWIZZLE_128B)
-         : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
+  if (kn ? !tmap_2d(&tb, u8, 1, B, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, (uint32_t)(pn / 2), BG_BK, pn == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)
+         : !tmap_2d(&tb, u8, 1, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, BG_BK, (uint32_t)(pn / 2), CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   if (p.n_tma == 0) tc = ta;
   else if (!tmap_2d(&tc, ct, esz, C, (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 128 / esz, 32, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   if (tiles < units) units = (int)tiles;
-  return cuda_status(kn ? launch_bg<true>(ta, tb, tc, p, dev, units, nullptr, st) : launch_bg<false>(ta, tb, tc, p, dev, units, nullptr, st),
-                     "block-scaled gemm launch");
+  return cuda_status(launch_bg_form(pn, kn, ta, tb, tc, p, dev, units, nullptr, st), "block-scaled gemm launch");
 }
 
 }  // namespace gsb

@@ -132,7 +132,8 @@ def check_gemm(c, a, b, sa, sb, transposed):
 
 
 GEMM_SIZES = [(1, 8, 128), (1, 2048, 512), (3, 130, 127), (7, 1, 1), (64, 384, 1000), (128, 256, 128), (129, 257, 129), (333, 1536, 512), (1000, 72, 2049),
-              (300, 129, 100), (20, 4096, 4096), (2500, 520, 640), (600, 1000, 300), (600, 1000, 2300), (5000, 1001, 520), (20000, 520, 384)]
+              (300, 129, 100), (20, 4096, 4096), (2500, 520, 640), (600, 1000, 300), (600, 1000, 2300), (5000, 1001, 520), (20000, 520, 384),
+              (1, 1000, 4097), (2, 72, 5120), (3, 513, 1000), (4, 1024, 2048), (5, 40, 300), (2, 9, 10240), (1, 16, 12000), (30000, 128, 200), (20001, 130, 700), (12000, 384, 384)]
 
 
 @pytest.mark.parametrize("transposed", [False, True])
