@@ -258,51 +258,60 @@ __device__ __forceinline__ float values_and_max(const Raw8<T>& r, float (&v)[8])
 // half-warp.  Rows are walked from the last to the first, as the other quantisers do (the consumer reads upwards and finds in L2
 // what was written last).
 struct RowWalk {
-  long long row;
-  int blk, blk_step;                    // this half-warp's blocks
-  __device__ __forceinline__ RowWalk(int nb) {
+  long long row;                        // the first; the others row_step apart
+  int row_step, blk, blk_step;          // this half-warp's blocks
+  __device__ __forceinline__ RowWalk(int nb, int rows = 1) {
     const int half = (threadIdx.x >> 4) & 1;
-    const long long w = (long long)(gridDim.x - 1 - blockIdx.x) * B8_WARPS + (threadIdx.x >> 5);
-    if (nb == 1) { row = 2 * w + half; blk = 0; blk_step = 1; }
-    else { row = w; blk = half; blk_step = 2; }
+    const long long w = ((long long)(gridDim.x - 1 - blockIdx.x) * B8_WARPS + (threadIdx.x >> 5)) * rows;
+    if (nb == 1) { row = 2 * w + half; row_step = 2; blk = 0; blk_step = 1; }
+    else { row = w; row_step = 1; blk = half; blk_step = 2; }
+  }
+  // Row j, or the last one where there are not so many (all lanes take part in the shuffles)
+  __device__ __forceinline__ long long in(int j, long long M) const {
+    const long long r = row + j * row_step;
+    return r < M ? r : M - 1;
   }
 };
-static long long row_walk_blocks(long long M, int nb) {
-  const long long rows = B8_WARPS * (nb == 1 ? 2 : 1);
+static long long row_walk_blocks(long long M, int nb, int rows_per_warp = 1) {
+  const long long rows = (long long)B8_WARPS * rows_per_warp * (nb == 1 ? 2 : 1);
   return (M + rows - 1) / rows;
 }
 
 // ---- quantise, a block per row ---------------------------------------------------------------------------------------------
-// NV blocks of a half-warp are loaded before the first is used.
-template <typename T, int V, int NV>
+// A warp takes ROWS rows (or pairs of one-block rows) at a time, and all NV blocks of a half-warp in each are loaded before the first is used: four
+// vectors in flight per lane.
+template <typename T, int V, int NV, int ROWS>
 __global__ void __launch_bounds__(B8_WARPS * 32)
 block_quantize_kernel(const T* x, long long ldx, uint8_t* q, long long ldq, float* scale, long long lds, long long M, int K) {
   const int nb = (K + B8 - 1) / B8, sub = threadIdx.x & 15;
-  const RowWalk w(nb);
+  const RowWalk w(nb, ROWS);
   pdl_wait();
   pdl_trigger();
-  const long long row = w.row < M ? w.row : M - 1;                 // (all lanes take part in the shuffles)
-  const bool mine = w.row < M;
-  const T* xr = x + row * ldx;
-  uint8_t* qr = q + row * ldq;
-  float* sr = scale + row * lds;
-  const long long room = row + 1 < M ? ldx : K;
   for (int b0 = 0; b0 < nb; b0 += NV * w.blk_step) {
-    Raw8<T> raw[NV];
+    Raw8<T> raw[ROWS][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = load_row8<T, V>(xr, (b0 + w.blk + i * w.blk_step) * B8 + sub * 8, K);
+    for (int j = 0; j < ROWS; ++j) {
+      const T* xr = x + w.in(j, M) * ldx;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) tail_row8<T, V>(raw[i], xr, (b0 + w.blk + i * w.blk_step) * B8 + sub * 8, K, room);
+      for (int i = 0; i < NV; ++i) raw[j][i] = load_row8<T, V>(xr, (b0 + w.blk + i * w.blk_step) * B8 + sub * 8, K);
+    }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int b = b0 + w.blk + i * w.blk_step;
-      float v[8];
-      float m = values_and_max<T>(raw[i], v);
-      if (__any_sync(0xffffffffu, m > FMAX)) m = finite_half_warp_max(v);
-      const float s = block_scale(m);
-      if (mine && b < nb) {
-        store_q8<V>(qr, b * B8 + sub * 8, K, to_e4m3(v, pow2_reciprocal(s)));
-        if (sub == 0) sr[b] = s;
+    for (int j = 0; j < ROWS; ++j) {
+      const long long row = w.in(j, M);
+      const bool mine = w.row + j * w.row_step < M;
+      const long long room = row + 1 < M ? ldx : K;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int b = b0 + w.blk + i * w.blk_step;
+        tail_row8<T, V>(raw[j][i], x + row * ldx, b * B8 + sub * 8, K, room);
+        float v[8];
+        float m = values_and_max<T>(raw[j][i], v);
+        if (__any_sync(0xffffffffu, m > FMAX)) m = finite_half_warp_max(v);
+        const float s = block_scale(m);
+        if (mine && b < nb) {
+          store_q8<V>(q + row * ldq, b * B8 + sub * 8, K, to_e4m3(v, pow2_reciprocal(s)));
+          if (sub == 0) scale[row * lds + b] = s;
+        }
       }
     }
   }
@@ -562,11 +571,14 @@ int32_t launch_block_quantize(const void* x, int dt, long long ldx, uint8_t* q, 
     return cuda_status(GSB_BY_TYPE(dt, CALL), "block quantise launch");
 #undef CALL
   }
-  const long long blocks = row_walk_blocks(M, nb);
+  // Several short rows a warp once they fill the SMs all the same (us, one row / several, bf16: M = 65536, K = 128 9.2 / 5.5, K = 512 18.9 / 16.3; M = 333,
+  // K = 512 1.4 / 1.9)
+  const bool many = M >= 16384;
+  const long long blocks = row_walk_blocks(M, nb, !many || nb > 4 ? 1 : nb <= 2 ? 4 : 2);
   if (!grid_fits(blocks)) return GSB200_ERR_BAD_ARG;
-#define CALL(T) launch_dependent(nb <= 2 ? GSB_BY_V(v, block_quantize_kernel, T, 1)      \
-                                 : nb <= 4 ? GSB_BY_V(v, block_quantize_kernel, T, 2)    \
-                                           : GSB_BY_V(v, block_quantize_kernel, T, 4),   \
+#define CALL(T) launch_dependent(nb <= 2 ? (many ? GSB_BY_V(v, block_quantize_kernel, T, 1, 4) : GSB_BY_V(v, block_quantize_kernel, T, 1, 1))   \
+                                 : nb <= 4 ? (many ? GSB_BY_V(v, block_quantize_kernel, T, 2, 2) : GSB_BY_V(v, block_quantize_kernel, T, 2, 1)) \
+                                           : GSB_BY_V(v, block_quantize_kernel, T, 4, 1),                                                       \
                                  (unsigned)blocks, B8_WARPS * 32, 0, st, static_cast<const T*>(x), ldx, q, ldq, scale, lds, M, K)
   return cuda_status(GSB_BY_TYPE(dt, CALL), "block quantise launch");
 #undef CALL

@@ -74,6 +74,18 @@ def test_quantize_at_the_borders_of_the_scale(dt):
         check_quantized(q, s, x, rows)
 
 
+@pytest.mark.parametrize("k", [100, 128, 250, 512, 300])
+@pytest.mark.parametrize("dt", TYPES)
+def test_quantize_many_short_rows(k, dt):
+    g = need_lib()
+    gen = torch.Generator().manual_seed(k)
+    x = rnd(gen, 16391, k).to(dt)
+    check_quantized(*g.fp8_block_quantize(x.cuda()), x, 1)
+    pad = torch.zeros(16391, (k + 7) // 8 * 8, dtype=dt, device="cuda")[:, :k]
+    pad.copy_(x)
+    check_quantized(*g.fp8_block_quantize(pad), x, 1)
+
+
 def test_quantize_every_half():
     g = need_lib()
     x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.float16).view(512, 128).clone()
