@@ -26,17 +26,21 @@ namespace gsb {
 constexpr int WG_BK = 256, WG_BM = 64;                     // columns of x^ (a pair's), rows per step
 constexpr int WG_WARPS = 8, WG_FRONT = 4, WG_THREADS = 32 * (WG_WARPS + WG_FRONT);
 constexpr int WG_CHUNK = WG_BM * 128;                      // a 64-column chunk of an operand tile: 64 rows of 128 bytes
-// Steps that the tensor core sums by itself.  Its fp32 additions truncate: over 8192 rows the sums are off by some 3.5e-6 (2-norm; plain fp32 sums 2e-7),
-// and it grows with the rows; longer parts are added to dW every so many steps, in fp32 as the parts are.
-constexpr int WG_SEG = 128;
+// Steps of 64 rows that the tensor core sums by itself.  Its fp32 additions truncate, which takes a little off a sum with each, fp16's longer products
+// more than bf16's: M = 65536, N = 2048, K = 512, bf16 comes out 3.2e-6 off (2-norm) from parts of 114 steps, 1.35e-6 from segments of 64, 9.8e-7 from 48,
+// 6e-7 from 32 (plain fp32 sums: 2e-7); M = 9001, fp16 1.2e-6 from 24.  It grows with the steps, so long parts are added to dW in segments, in fp32 as
+// the parts are.  Each costs 7 us, the time of 256 KiB per CTA through L2 (without 105 us, segments of 64 114, of 32 130; written by the threads instead of
+// by TMA 120 and 167).
+template <typename T> constexpr int WG_SEGMENT = std::is_same<T, __half>::value ? 64 : 128;
 constexpr int WG_AHEAD = 4;                                // steps of x^ in flight to the registers
 constexpr int WG_B_BYTES = 2 * WG_CHUNK;                   // a CTA's 128 columns of x^
 template <int ACC>                                         // accumulators (128 rows of dW per CTA each)
 struct WgSmem {
   static constexpr int A_BYTES = ACC * 2 * WG_CHUNK;
   static constexpr int STAGE = A_BYTES + WG_B_BYTES;       // 48 or 32 KiB
-  static constexpr int STAGES = ACC == 2 ? 4 : 6;
-  static constexpr int BAR = STAGES * STAGE;
+  static constexpr int STAGES = ACC == 2 ? 4 : 5;
+  static constexpr int OUT = STAGES * STAGE;               // per warp a box of 32 rows x 32 columns of dW
+  static constexpr int BAR = OUT + WG_WARPS * 4096;
   static constexpr int BYTES = BAR + 256 + 1024;
   static_assert(BYTES <= 227 * 1024, "shared memory budget");
 };
@@ -44,7 +48,8 @@ struct WgSmem {
 struct WgParams {
   const uint8_t* q; long long ldq; const float* s; long long lds;
   float* out; long long ldo;                               // dW, or this part's sums in the workspace
-  long long part_stride;                                   // elements between the parts
+  long long part_rows;                                     // rows between the parts
+  int tma_out;                                             // dW goes out in boxes
   long long M; int N, K, k_tiles, tiles, steps, parts;     // steps of 64 rows in all
   int accumulate;
 };
@@ -75,19 +80,13 @@ __device__ __forceinline__ void restore16<__nv_bfloat16>(uint4 r, float s, uint4
   lo = make_uint4(o[0], o[1], o[2], o[3]); hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// Sums of four floats held as words
-__device__ __forceinline__ uint4 add4(uint4 a, uint4 b) {
-  return make_uint4(__float_as_uint(__uint_as_float(a.x) + __uint_as_float(b.x)), __float_as_uint(__uint_as_float(a.y) + __uint_as_float(b.y)),
-                    __float_as_uint(__uint_as_float(a.z) + __uint_as_float(b.z)), __float_as_uint(__uint_as_float(a.w) + __uint_as_float(b.w)));
-}
-
 template <typename T, int ACC>
 __global__ void __launch_bounds__(WG_THREADS, 1)
-wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
+wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_out, const WgParams p) {
   extern __shared__ uint8_t wg_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wg_smem_raw) + 1023) & ~uintptr_t(1023));
   using L = WgSmem<ACC>;
-  constexpr int STAGES = L::STAGES;
+  constexpr int STAGES = L::STAGES, WG_SEG = WG_SEGMENT<T>;
   uint64_t* full_a = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* full_b = full_a + STAGES;
   uint64_t* empty = full_b + STAGES;
@@ -106,7 +105,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
     mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS);
     abort_flag.set(0);
     fence_mbar_init();
-    prefetch_tmap(&tm_dy);
+    prefetch_tmap(&tm_dy); prefetch_tmap(&tm_out);
   }
   if (warp == 1) { tmem_alloc_pair(tmem_slot, 256 * ACC); tmem_relinquish_pair(); }
   pdl_wait();
@@ -216,28 +215,31 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full, seg & 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF40, budget))) { ok = false; return; }
       tc_fence_after();
       const uint32_t t = tmem_base + (ACC == 2 ? 256 * half : cb) + ((uint32_t)(q * 32) << 16);
-      float* o = p.out + part * p.part_stride + (long long)n * p.ldo + k0 + cb;
-      const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * 4) | (uintptr_t)(p.part_stride * 4)) & 31) == 0;
       const bool add = p.accumulate || seg > 0;
+      uint8_t* const box = smem + L::OUT + (warp - WG_FRONT) * 4096;
+      float* o = p.out + (part * p.part_rows + n) * p.ldo + k0 + cb;
+      if (seg > 0 && lane == 0) tma_store_wait_all<0>();   // the segment before is in memory
       for (int c0 = 0; c0 < COLS && k0 + cb + c0 < p.K; c0 += 32) {
         uint32_t v[32];
         __syncwarp();
         tmem_ld_32x32b_x32(t + c0, v);
         tmem_ld_wait(v);
-        float* oc = o + c0;
-        if (n < p.N && wide && k0 + cb + c0 + 32 <= p.K) {
+        if (p.tma_out) {
+          if (lane == 0) tma_store_wait_read<0>();         // the previous box has left the buffer
+          __syncwarp();
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint4 x = make_uint4(v[8 * b], v[8 * b + 1], v[8 * b + 2], v[8 * b + 3]), y = make_uint4(v[8 * b + 4], v[8 * b + 5], v[8 * b + 6], v[8 * b + 7]);
-            if (add) {
-              uint4 ox, oy;
-              ldg_v8(oc + 8 * b, ox, oy);
-              x = add4(x, ox);
-              y = add4(y, oy);
-            }
-            stg_v8(oc + 8 * b, x, y);
+          for (int pc = 0; pc < 8; ++pc)
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((pc ^ (lane & 7)) << 4)) = make_uint4(v[4 * pc], v[4 * pc + 1], v[4 * pc + 2], v[4 * pc + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int x = k0 + cb + c0, y = (int)(part * p.part_rows) + n;     // (lane 0's n: the warp's first row)
+            if (add) tma_add_f32_2d(&tm_out, box, x, y);
+            else tma_store_2d(&tm_out, box, x, y);
+            tma_store_commit();
           }
         } else if (n < p.N) {
+          float* oc = o + c0;
 #pragma unroll
           for (int b = 0; b < 32; ++b)
             if (k0 + cb + c0 + b < p.K) oc[b] = add ? oc[b] + __uint_as_float(v[b]) : __uint_as_float(v[b]);
@@ -245,10 +247,11 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
       }
     };
     const uint32_t drained = mapa_shared(smem_u32(acc_empty), 0);
-    static_assert(WG_SEG % WG_AHEAD == 0, "a segment is whole rounds of the loop below");
+    static_assert(WG_SEG % WG_AHEAD == 0 && WG_AHEAD <= STAGES, "a segment is whole rounds of the loop below, and a round fits the ring");
     int s = 0; uint32_t ph = 0;
     for (int i0 = step0; ok && i0 < step1; i0 += WG_AHEAD) {
-      if (i0 != step0 && (i0 - step0) % WG_SEG == 0) {
+      // (the next segment's first steps are in shared memory before: its MMAs start as soon as the sums are out)
+      if (i0 - step0 > WG_SEG && (i0 - step0) % WG_SEG == WG_AHEAD) {
         drain((i0 - step0) / WG_SEG - 1);
         if (!ok) break;
         tc_fence_before();
@@ -279,7 +282,16 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const WgParams p) {
         if (++s == STAGES) { s = 0; ph ^= 1; }
       }
     }
-    if (ok) drain((step1 - step0 - 1) / WG_SEG);
+    // (the last segment; and the one before it, if this one was too short to come to that above)
+    const int last = (step1 - step0 - 1) / WG_SEG;
+    if (ok && last > 0 && step1 - step0 - last * WG_SEG <= WG_AHEAD) {
+      drain(last - 1);
+      tc_fence_before();
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive_remote(drained);
+    }
+    if (ok) drain(last);
+    if (lane == 0) tma_store_wait_all<0>();
   }
   tc_fence_before();
   cluster_sync_all();                                      // neither CTA leaves while the other may still arrive at its barriers or its MMAs read here
@@ -313,7 +325,7 @@ __global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long par
 // 10.1 / 13.9, 3000 18.8 / 22.5, 9001 30.0 / 29.4, 65536 137 / 104; N = 512 M = 9001 16.8 / 22.5, 65536 43.6 / 42.1): two from 14 steps a part.  A function of the
 // sizes alone: a workspace asked for before a device is chosen fits, and the sums have the same order everywhere.
 constexpr int WG_FILL = 74;
-static void wgrad_plan(long long M, int N, int K, int& acc, int& tiles, int& steps, int& parts, long long& ld, long long& part_stride) {
+static void wgrad_plan(long long M, int N, int K, int& acc, int& tiles, int& steps, int& parts, long long& ld, long long& part_rows) {
   const int kt = (K + WG_BK - 1) / WG_BK;
   steps = (int)((M + WG_BM - 1) / WG_BM);
   for (acc = N > 256 ? 2 : 1; ; acc = 1) {
@@ -324,7 +336,7 @@ static void wgrad_plan(long long M, int N, int K, int& acc, int& tiles, int& ste
     if (acc == 1 || steps >= 14 * parts) break;
   }
   ld = ((long long)K + 7) / 8 * 8;
-  part_stride = ld * N;
+  part_rows = (long long)(N + 256 * acc - 1) / (256 * acc) * (256 * acc);      // (whole tiles: what lies behind N stays in its part)
 }
 static bool wgrad_shape_ok(long long M, int N, int K) {
   return M >= 0 && M <= 0x7fffff00ll && N > 0 && K > 0 && N <= (1 << 24) && K <= (1 << 24) &&
@@ -332,13 +344,13 @@ static bool wgrad_shape_ok(long long M, int N, int K) {
 }
 int64_t wgrad_workspace_bytes(long long M, int N, int K) {
   if (!wgrad_shape_ok(M, N, K)) return 0;
-  int acc, tiles, steps, parts; long long ld, stride;
-  wgrad_plan(M, N, K, acc, tiles, steps, parts, ld, stride);
-  return parts > 1 ? 4 * stride * parts : 0;
+  int acc, tiles, steps, parts; long long ld, rows;
+  wgrad_plan(M, N, K, acc, tiles, steps, parts, ld, rows);
+  return parts > 1 ? 4 * ld * rows * parts : 0;
 }
 
 template <typename T, int ACC>
-static cudaError_t launch_wg(const CUtensorMap& tm, const WgParams& p, int dev, unsigned grid, cudaStream_t st) {
+static cudaError_t launch_wg(const CUtensorMap& tm, const CUtensorMap& to, const WgParams& p, int dev, unsigned grid, cudaStream_t st) {
   static std::atomic<int> attr_done[64];
   auto k = wgrad_kernel<T, ACC>;
   if (!attr_done[dev].load(std::memory_order_acquire)) {
@@ -354,7 +366,7 @@ static cudaError_t launch_wg(const CUtensorMap& tm, const WgParams& p, int dev, 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid); cfg.blockDim = dim3(WG_THREADS); cfg.dynamicSmemBytes = WgSmem<ACC>::BYTES; cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k, tm, p);
+  return cudaLaunchKernelEx(&cfg, k, tm, to, p);
 }
 
 int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, long long ldq, const float* s, long long lds, float* dw, long long lddw,
@@ -372,8 +384,8 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
   if (rc != GSB200_OK) return rc;
   WgParams p{};
   int acc;
-  long long ld, stride;
-  wgrad_plan(M, N, K, acc, p.tiles, p.steps, p.parts, ld, stride);
+  long long ld, rows;
+  wgrad_plan(M, N, K, acc, p.tiles, p.steps, p.parts, ld, rows);
   const long long need = wgrad_workspace_bytes(M, N, K);
   if (need > 0 && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 31))) return GSB200_ERR_BAD_ARG;
   int dev = 0;
@@ -384,16 +396,21 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
                (uint64_t)lddy, 64, WG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   p.q = q; p.ldq = ldq; p.s = s; p.lds = lds; p.M = M; p.N = N; p.K = K; p.k_tiles = (K + WG_BK - 1) / WG_BK;
   const bool cut = p.parts > 1;
-  p.out = cut ? static_cast<float*>(ws) : dw; p.ldo = cut ? ld : lddw; p.part_stride = cut ? stride : 0;
+  p.out = cut ? static_cast<float*>(ws) : dw; p.ldo = cut ? ld : lddw; p.part_rows = cut ? rows : 0;
+  // (TMA writes whole 16-byte pieces)
+  p.tma_out = cut || ((reinterpret_cast<uintptr_t>(dw) & 15) == 0 && lddw % 4 == 0 && K % 4 == 0);
   p.accumulate = cut ? 0 : accumulate;
+  CUtensorMap to = tm;
+  if (p.tma_out && !tmap_2d(&to, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.out, (uint64_t)(cut ? rows * p.parts : N), (uint64_t)(cut ? ld : K), (uint64_t)p.ldo, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   const long long grid = 2ll * p.tiles * p.parts;
   if (grid > 0x7fffffffll) return GSB200_ERR_BAD_ARG;
   const bool f16 = dt == GSB200_F16;
-  cudaError_t e = acc == 2 ? (f16 ? launch_wg<__half, 2>(tm, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 2>(tm, p, dev, (unsigned)grid, st))
-                           : (f16 ? launch_wg<__half, 1>(tm, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 1>(tm, p, dev, (unsigned)grid, st));
+  cudaError_t e = acc == 2 ? (f16 ? launch_wg<__half, 2>(tm, to, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 2>(tm, to, p, dev, (unsigned)grid, st))
+                           : (f16 ? launch_wg<__half, 1>(tm, to, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 1>(tm, to, p, dev, (unsigned)grid, st));
   if (e == cudaSuccess && cut) {
     const long long n4 = (long long)N * ((K + 3) / 4);
-    e = launch_dependent(wgrad_reduce_kernel, (unsigned)((n4 + 255) / 256), 256, 0, st, static_cast<const float*>(ws), ld, stride, p.parts, dw, lddw, N, K, accumulate);
+    e = launch_dependent(wgrad_reduce_kernel, (unsigned)((n4 + 255) / 256), 256, 0, st, static_cast<const float*>(ws), ld, rows * ld, p.parts, dw, lddw, N, K, accumulate);
   }
   return cuda_status(e, "weight gradient launch");
 }
