@@ -666,13 +666,14 @@ int32_t launch_block_gemm(const uint8_t* A, long long lda, const float* sa, long
     const long long rb2 = (M + 2 * BG_BM - 1) / (2 * BG_BM);
     // 128 columns where their rounds are cheaper: a tile takes 0.57 of the time of a 256-column one up to K = 512, 0.69 from there on (us, 256 / 128
     // columns, M = 65536: K = 512 N = 128 16.0 / 12.9, 640 41.0 / 40.4, 1536 70.6 / 80.2; K = 384, N = 384 25.9 / 23.4; K = 2048, N = 512 71.1 / 98.5)
-    const long long r256 = (rb2 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2 > 0 ? sms / 2 : 1), r128 = (rb2 * nb + sms / 2 - 1) / (sms / 2 > 0 ? sms / 2 : 1);
+    const long long pairs = sms / 2 > 0 ? sms / 2 : 1;
+    const long long r256 = (rb2 * ((N + 255) / 256) + pairs - 1) / pairs, r128 = (rb2 * nb + pairs - 1) / pairs;
     if (r128 * (kb <= 4 ? 60 : 69) < r256 * 100) pn = 128;
     int cap = 0;
     const cudaError_t e = launch_bg_form(pn, kn, ta, ta, ta, p, dev, 0, &cap, st);
     if (e != cudaSuccess) return cuda_status(e, "block-scaled gemm set-up");
-    units = sms / 2 < cap ? sms / 2 : cap;
-    if (units == 0) bn = 128;
+    units = (int)(pairs < cap ? pairs : cap);
+    if (units == 0) bn = 128;                                // (pairs cannot be launched here)
   }
   if (bn != 0) {
     p.m_blocks = (int)rb; p.n_blocks = (N + bn - 1) / bn;

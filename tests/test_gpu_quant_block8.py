@@ -224,6 +224,34 @@ def test_gemm_what_lies_behind_the_operands_rows_does_not_matter():
         assert torch.equal(got, ref)
 
 
+@pytest.mark.parametrize("limit", [1, 9, 60])
+def test_gemm_under_an_sm_limit(limit):
+    """Fewer CTAs than tiles: the same bytes."""
+    g = need_lib()
+    sets = [operands(torch.Generator().manual_seed(5), m, n, k, tr) + (tr,) for m, n, k, tr in ((700, 400, 300, False), (2100, 520, 260, True), (40, 700, 512, False))]
+    ref = [g.gemm_fp8_block(a, b, sa, sb, b_transposed=tr) for a, b, sa, sb, tr in sets]
+    g.lib().gsb200_set_sm_limit(limit)
+    try:
+        got = [g.gemm_fp8_block(a, b, sa, sb, b_transposed=tr) for a, b, sa, sb, tr in sets]
+        torch.cuda.synchronize()
+    finally:
+        g.lib().gsb200_set_sm_limit(0)
+    assert all(torch.equal(x, y) for x, y in zip(got, ref)) and g.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+def test_gemm_rows_do_not_depend_on_the_form(m):
+    """A row's result is the same whichever kernel the number of rows selects, up to the order of fp32 sums."""
+    g = need_lib()
+    a, b, sa, sb = operands(torch.Generator().manual_seed(m), 300, 264, 1000, False)
+    for dt in TYPES:
+        full = g.gemm_fp8_block(a, b, sa, sb, dtype=dt)
+        _, mag = block8.gemm(a[:m], sa[:m], b, sb)
+        few = g.gemm_fp8_block(a[:m], b, sa[:m], sb, dtype=dt)
+        tol = 2 * eps(dt) * full[:m].double().abs() + 2 * (128 + 11) * 2.0 ** -23 * mag + 2.0 ** -24
+        assert bool(((few.double() - full[:m].double()).abs() <= tol).all())
+
+
 # ---- weight gradient -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 128), (1, 1, 1), (63, 130, 127), (64, 256, 256), (65, 129, 257), (300, 1000, 520), (2000, 512, 100), (5000, 264, 512),
