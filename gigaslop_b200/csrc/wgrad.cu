@@ -298,8 +298,9 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
   if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem_base, 256 * ACC); }
 }
 
-// dW = (dW +) the parts' sums, in order.
-__global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long part_stride, int parts, float* out, long long ldo, int N, int K, int accumulate) {
+// dW = (dW +) the parts' sums, in order.  A thread's loads are what it waits for: eight parts' at a time, dW as vectors where its rows allow
+// (accumulating, scalar by scalar / so: N = 2048 K = 512 M = 9001 29.8 / 28.5 us, N = 512 16.7 / 15.7).
+__global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long part_stride, int parts, float* out, long long ldo, int N, int K, int accumulate, int vec) {
   const int per_row = (K + 3) / 4;
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   pdl_wait();
@@ -307,17 +308,29 @@ __global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long par
   const int n = (int)(i / per_row), k = (int)(i % per_row) * 4;
   const float* w = ws + (long long)n * ld + k;            // (the workspace's rows are padded to whole vectors)
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j = 0; j < parts; ++j) {
+  int j = 0;
+  for (; j + 8 <= parts; j += 8) {                        // eight parts' loads in flight
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const float4*>(w + (j + u) * part_stride);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) { a.x += v[u].x; a.y += v[u].y; a.z += v[u].z; a.w += v[u].w; }
+  }
+#pragma unroll 4
+  for (; j < parts; ++j) {
     const float4 v = *reinterpret_cast<const float4*>(w + j * part_stride);
     a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
   }
+  float* o = out + (long long)n * ldo + k;
+  if (vec) {                                              // (dW's rows are whole aligned vectors)
+    float4 d = accumulate ? *reinterpret_cast<const float4*>(o) : make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<float4*>(o) = accumulate ? make_float4(d.x + a.x, d.y + a.y, d.z + a.z, d.w + a.w) : a;
+    return;
+  }
   const float e[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (k + j < K) {
-      float* o = out + (long long)n * ldo + k + j;
-      *o = accumulate ? *o + e[j] : e[j];
-    }
+  for (int u = 0; u < 4; ++u)
+    if (k + u < K) o[u] = accumulate ? o[u] + e[u] : e[u];
 }
 
 // Accumulators per CTA, tiles, and the parts the batch is cut into: what fills the SMs with pairs, at least four steps each.  Two accumulators use
@@ -410,7 +423,8 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
                            : (f16 ? launch_wg<__half, 1>(tm, to, p, dev, (unsigned)grid, st) : launch_wg<__nv_bfloat16, 1>(tm, to, p, dev, (unsigned)grid, st));
   if (e == cudaSuccess && cut) {
     const long long n4 = (long long)N * ((K + 3) / 4);
-    e = launch_dependent(wgrad_reduce_kernel, (unsigned)((n4 + 255) / 256), 256, 0, st, static_cast<const float*>(ws), ld, rows * ld, p.parts, dw, lddw, N, K, accumulate);
+    const int vec = (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && lddw % 4 == 0 && K % 4 == 0;
+    e = launch_dependent(wgrad_reduce_kernel, (unsigned)((n4 + 255) / 256), 256, 0, st, static_cast<const float*>(ws), ld, rows * ld, p.parts, dw, lddw, N, K, accumulate, vec);
   }
   return cuda_status(e, "weight gradient launch");
 }
