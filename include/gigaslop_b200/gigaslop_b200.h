@@ -258,10 +258,12 @@ int32_t gsb200_block_dequantize_fp8(const uint8_t* q, int64_t ldq, const float* 
                                     int64_t ldx, int64_t M, int32_t K, int32_t block_rows, gsb200_stream_t stream);
 
 /* C[m,n] = sum over blocks b of scale_a[m,b] * scale_b[n/128,b] * (sum over k in b of A[m,k] B[n,k]): fp32 sums, one rounding to C's type.
- * A [M,K] with scales per row and block, B [N,K] with scales per tile; any fp32 scales whose products are finite.  One row to many.
+ * A [M,K] with scales per row and block, B [N,K] with scales per tile; any fp32 scales whose products neither overflow nor (but for zero)
+ * fall below 2^-126.  One row to many.
  * flags = GSB200_FLAG_B_KN: B is [K,N] with scale_b[k/128, n/128].  That is the input gradient dX = dY . W with W and its scales as the
  * forward pass has them (A = the quantised dY, K = the layer's outputs, N = its inputs).  C: any alignment (16-byte rows are the
- * fast ones). */
+ * fast ones).  Under gsb200_set_sm_limit as the other GEMMs, except that one pair of CTAs is the least, and that products of up to four rows on
+ * [N,K] know no limit (small CTAs, beside which others run). */
 int32_t gsb200_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* scale_a, int64_t ld_scale_a, const uint8_t* B, int64_t ldb,
                               const float* scale_b, int64_t ld_scale_b, void* C, int64_t ldc, int32_t c_dtype, int64_t M, int32_t N,
                               int32_t K, int32_t flags, gsb200_stream_t stream);
@@ -270,6 +272,7 @@ int32_t gsb200_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* scale_
  * accumulate != 0 adds to what dW holds (gradient accumulation).  dY fp16 or bf16 [M,N], q / scale as the forward pass's quantiser left
  * them [M,K].  q * scale is rounded to dY's type on its way to the tensor cores: exact for scales that are powers of two (fp16: and values
  * up to 65504).  The order of the sums depends on the sizes alone.  M = 0 gives zeros (or leaves dW as it is).
+ * N and K up to 2^24 (2^24 tiles of 256 x 256).  A CTA ends with its tile: no gsb200_set_sm_limit.
  * workspace: gsb200_gemm_fp8_block_wgrad_workspace_bytes(M, N, K) bytes (may be 0), 32-byte aligned; calls that may overlap
  * need one each. */
 int64_t gsb200_gemm_fp8_block_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K);
@@ -279,6 +282,7 @@ int32_t gsb200_gemm_fp8_block_wgrad(const void* dY, int32_t dy_dtype, int64_t ld
 
 /* SwiGLU into the format, with checkpoints: h = gate * sigmoid(gate) * up in fp32, quantised from there (the down-projection's operand), and
  * gate and up quantised for the backward pass.  gate, up [M,F] of one type; the three outputs share their row strides.
+ * The sigmoid is taken in fp32: below gate = -87 it may be 0.
  * The gradient reads the checkpoints (any scales): with s = sigmoid(gate), dup = dh * gate * s, dgate = dh * up * s * (1 + gate * (1 - s)), in
  * dh's type.  dgate_q .. dup_s (all four or none): the two gradients quantised as well, from their rounded values, for the input gradient's
  * product. */

@@ -276,6 +276,44 @@ def test_wgrad(m, n, k, dt):
     assert g.device_status()[0] == 0
 
 
+@pytest.mark.parametrize("dt,m", [(torch.float16, 4100), (torch.float16, 8250), (torch.bfloat16, 8250)])
+@pytest.mark.parametrize("k,ld", [(1000, 1000), (1000, 1004), (1001, 1001)])
+def test_wgrad_in_segments_straight_to_dw(k, ld, dt, m):
+    """So many tiles that the batch is not cut: its segments are added in dW itself, in boxes or element by element, to what it holds or not."""
+    g = need_lib()
+    gen = torch.Generator().manual_seed(m + ld)
+    n = 9700
+    assert g.lib().gsb200_gemm_fp8_block_wgrad_workspace_bytes(m, n, k) == 0
+    q, s = g.fp8_block_quantize(rnd(gen, m, k).cuda())
+    dy = (rnd(gen, m, 9704) * 0.1).to(dt).cuda()[:, :n]
+    want, mag = block8.wgrad(dy, q, s)
+    tol = eps(torch.float32) * want.abs() + (m + 160) * 2.0 ** -23 * mag
+    buf = torch.full((n, ld), math.nan, device="cuda")
+    dw = g.gemm_fp8_block_wgrad(dy, q, s, out=buf[:, :k])
+    assert bool(((dw.double() - want).abs() <= tol).all()) and bool(buf[:, k:].isnan().all())
+    start = dw.double()
+    g.gemm_fp8_block_wgrad(dy, q, s, out=dw, accumulate=True)
+    want = want + start
+    assert bool(((dw.double() - want).abs() <= tol + 3 * 2.0 ** -23 * (want.abs() + mag)).all()) and bool(buf[:, k:].isnan().all())     # (up to three additions to dW)
+    assert g.device_status()[0] == 0
+
+
+def test_wgrad_and_few_rows_know_no_sm_limit():
+    g = need_lib()
+    gen = torch.Generator().manual_seed(4)
+    q, s = g.fp8_block_quantize(rnd(gen, 3000, 520).cuda())
+    dy = rnd(gen, 3000, 1000).half().cuda()
+    a, b, sa, sb = operands(gen, 2, 700, 512, False)
+    ref = [g.gemm_fp8_block_wgrad(dy, q, s), g.gemm_fp8_block(a, b, sa, sb)]
+    g.lib().gsb200_set_sm_limit(1)
+    try:
+        got = [g.gemm_fp8_block_wgrad(dy, q, s), g.gemm_fp8_block(a, b, sa, sb)]
+        torch.cuda.synchronize()
+    finally:
+        g.lib().gsb200_set_sm_limit(0)
+    assert all(torch.equal(x, y) for x, y in zip(got, ref)) and g.device_status()[0] == 0
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_wgrad_any_scales(dt):
     """Scales that are no powers of two: the restored element is rounded to dY's type, once."""
@@ -399,6 +437,26 @@ def test_swiglu_far_gates_and_nan():
     dg, du = g.swiglu_fp8_block_bwd(torch.ones_like(gate), gq, gs, uq, us)
     assert bool(dg[:, 8].isnan().all()) and bool(torch.isfinite(dg[:, [i for i in range(12) if i != 8]]).all())
     assert bool((dg[:, 0] == 0).all()) and bool((dg[:, 7] == 1).all())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_swiglu_gates_where_the_sigmoid_leaves_fp32(dt):
+    """e^-g passes fp32's range at g = -88.7, and 1 / e^-g its normal numbers at -87.3: from there on the sigmoid may be 0 instead of its value, which is below
+    2^-125 (1.00001 of it).  Before that its exponent is rounded at |g| log2 e < 128: 2^-18 relative, and as much for the rest."""
+    g = need_lib()
+    gate = torch.linspace(-92, -80, 256).to(dt).repeat(2, 1).cuda()
+    up = torch.stack([torch.ones(256), torch.full((256,), 3e4)]).to(dt).cuda()
+    (hq, hs), (gq, gs), (uq, us) = g.swiglu_fp8_block(gate, up)
+    h, want = block8.values(hq, hs), block8.swiglu(gate.double(), up.double())
+    lost = (gate.double() * up.double()).abs() * 2.0 ** -125
+    assert bool(((h - want).abs() <= (2.0 ** -4 * want.abs()).maximum(2.0 ** -10 * block8.spread(hs, 1, 2, 256)) * (1 + 2.0 ** -15) + lost).all())
+    dh = torch.ones_like(gate)
+    wg, wu = block8.swiglu_bwd(dh.double(), block8.values(gq, gs), block8.values(uq, us))
+    dg, du = g.swiglu_fp8_block_bwd(dh, gq, gs, uq, us)
+    tiny = 2.0 ** -25 if dt == torch.float16 else 2.0 ** -133
+    gv, uv = block8.values(gq, gs), block8.values(uq, us)
+    for got, w, lost in ((dg, wg, (uv * (1 + gv.abs())).abs() * 2.0 ** -125), (du, wu, gv.abs() * 2.0 ** -125)):
+        assert bool(((got.double() - w).abs() <= (eps(dt) + 2.0 ** -16) * w.abs() + lost + tiny).all())
 
 
 def test_swiglu_views():
