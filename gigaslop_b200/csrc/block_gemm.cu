@@ -63,6 +63,25 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
   return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
+// Rows of C that no wide store may take: a warp's 32 rows of up to 128 bytes go through its 4 KiB box of shared memory, so that a store
+// covers one row's neighbours instead of a column of 32 rows (us, contiguous rows of fp16, element by element / so: M = 65536, N = 1535, K = 512 979 / 131; M = 371,
+// N = 3287, K = 640 23.1 / 6.1).  pieces(pc): 16-byte piece pc of this lane's row, NP of them.
+template <typename E, int NP, typename P>
+__device__ __forceinline__ void store_by_rows(uint8_t* box, int lane, P pieces, E* c, long long ldc, int rows, int cols) {
+  __syncwarp();
+#pragma unroll
+  for (int pc = 0; pc < NP; ++pc) *reinterpret_cast<uint4*>(box + lane * 128 + ((pc ^ (lane & 7)) << 4)) = pieces(pc);
+  __syncwarp();
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int x = lane; x < NP * 16 / (int)sizeof(E); x += 32) {
+      const int b = x * (int)sizeof(E);
+      if (x < cols) c[r * ldc + x] = *reinterpret_cast<const E*>(box + r * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15));
+    }
+  }
+}
+
 struct BgParams {
   int M, N, m_blocks, n_blocks, k_blocks;                  // a pair's row block is 256 rows, 128 per CTA
   const float* sa; long long ld_sa;
@@ -296,15 +315,32 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }, std::integral_constant<int, CW / 64>{}, n0, CW > 64 && tma_cols > 64 ? 2 : 1);
         }
       }
-      if (tma_cols < CW && p.n_tma < p.N && row < p.M) {       // what TMA cannot address, element by element
-        const long long o = (long long)row * p.ldc + n0;
+      if (tma_cols < CW && p.n_tma < p.N) {                    // what TMA cannot address (n_tma is a whole number of boxes)
+        if (lane == 0) tma_store_wait_read<0>();
+        const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
+        const long long o = (long long)m0 * p.ldc + n0;
+        if (p.c_type == GSB200_F32) {
 #pragma unroll
-        for (int i = 0; i < CW; ++i) {
-          if (i < tma_cols || n0 + i >= p.N) continue;
-          if (p.c_type == GSB200_F32) static_cast<float*>(p.C)[o + i] = acc[i];
-          else if (p.c_type == GSB200_F16) static_cast<__half*>(p.C)[o + i] = __float2half_rn(acc[i]);
-          else static_cast<__nv_bfloat16*>(p.C)[o + i] = __float2bfloat16_rn(acc[i]);
+          for (int c0 = 0; c0 < CW; c0 += 32) {
+            if (c0 < tma_cols || n0 + c0 >= p.N) continue;
+            store_by_rows<uint32_t, 8>(out_buf, lane, [&](int pc) {
+              const float* a = acc + c0 + 4 * pc;
+              return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+            }, static_cast<uint32_t*>(p.C) + o + c0, p.ldc, rows, p.N - n0 - c0);
+          }
+        } else {
+          const bool f16 = p.c_type == GSB200_F16;
+#pragma unroll
+          for (int c0 = 0; c0 < CW; c0 += 64) {
+            if (c0 < tma_cols || n0 + c0 >= p.N) continue;
+            store_by_rows<uint16_t, 8>(out_buf, lane, [&](int pc) {
+              const float* a = acc + c0 + 8 * pc;
+              return f16 ? make_uint4(pack_half2(a[0], a[1]), pack_half2(a[2], a[3]), pack_half2(a[4], a[5]), pack_half2(a[6], a[7]))
+                         : make_uint4(pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3]), pack_bf2(a[4], a[5]), pack_bf2(a[6], a[7]));
+            }, static_cast<uint16_t*>(p.C) + o + c0, p.ldc, rows, p.N - n0 - c0);
+          }
         }
+        __syncwarp();                                          // (the next tile's boxes go into the same buffer)
       }
     }
     if (lane == 0) tma_store_wait_all<0>();
@@ -446,23 +482,33 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
         if (++as == ACC) { as = 0; aph ^= 1; }
       }
     }
-    if (ok && live && row < p.M) {
-      const int esz = p.c_type == GSB200_F32 ? 4 : 2;
-      uint8_t* dst = static_cast<uint8_t*>(p.C) + ((long long)row * p.ldc + n) * esz;
-      const bool wide = ((reinterpret_cast<uintptr_t>(p.C) | (uintptr_t)(p.ldc * esz)) & 31) == 0;
-      if (p.c_type == GSB200_F32) {
+    const int esz = p.c_type == GSB200_F32 ? 4 : 2;
+    uint8_t* dst = static_cast<uint8_t*>(p.C) + ((long long)row * p.ldc + n) * esz;
+    // 32 or 16 bytes at a time, as C's rows allow (M = 371, N = 3288, K = 640, fp16: element by element 23.5 us, 16 bytes 5.2)
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.C) | (uintptr_t)(p.ldc * esz);
+    const bool wide = (at & 31) == 0;
+    if (ok && live && (at & 15) == 0) {
+      if (row < p.M && p.c_type == GSB200_F32) {
 #pragma unroll
         for (int b = 0; b < CW / 8; ++b) {
+          const uint4 v[2] = {make_uint4(__float_as_uint(acc[8 * b]), __float_as_uint(acc[8 * b + 1]), __float_as_uint(acc[8 * b + 2]), __float_as_uint(acc[8 * b + 3])),
+                              make_uint4(__float_as_uint(acc[8 * b + 4]), __float_as_uint(acc[8 * b + 5]), __float_as_uint(acc[8 * b + 6]), __float_as_uint(acc[8 * b + 7]))};
           if (wide && n + 8 * b + 8 <= p.N) {
-            stg_v8(dst + 32 * b, make_uint4(__float_as_uint(acc[8 * b]), __float_as_uint(acc[8 * b + 1]), __float_as_uint(acc[8 * b + 2]), __float_as_uint(acc[8 * b + 3])),
-                   make_uint4(__float_as_uint(acc[8 * b + 4]), __float_as_uint(acc[8 * b + 5]), __float_as_uint(acc[8 * b + 6]), __float_as_uint(acc[8 * b + 7])));
+            stg_v8(dst + 32 * b, v[0], v[1]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (n + 8 * b + i < p.N) reinterpret_cast<float*>(dst)[8 * b + i] = acc[8 * b + i];
+            for (int h = 0; h < 2; ++h) {
+              if (n + 8 * b + 4 * h + 4 <= p.N) {
+                *reinterpret_cast<uint4*>(dst + 32 * b + 16 * h) = v[h];
+              } else {
+#pragma unroll
+                for (int i = 4 * h; i < 4 * h + 4; ++i)
+                  if (n + 8 * b + i < p.N) reinterpret_cast<float*>(dst)[8 * b + i] = acc[8 * b + i];
+              }
+            }
           }
         }
-      } else {
+      } else if (row < p.M) {
 #pragma unroll
         for (int b = 0; b < CW / 16; ++b) {
           uint32_t w[8];
@@ -472,10 +518,40 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
             stg_v8(dst + 32 * b, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n + 16 * b + i < p.N) reinterpret_cast<uint16_t*>(dst)[16 * b + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+            for (int h = 0; h < 2; ++h) {
+              if (n + 16 * b + 8 * h + 8 <= p.N) {
+                *reinterpret_cast<uint4*>(dst + 32 * b + 16 * h) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+              } else {
+#pragma unroll
+                for (int i = 8 * h; i < 8 * h + 8; ++i)
+                  if (n + 16 * b + i < p.N) reinterpret_cast<uint16_t*>(dst)[16 * b + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+              }
+            }
           }
         }
+      }
+    } else if (ok && live) {                               // through the operands' memory: the last sums are here, so nothing reads or writes it any more
+      static_assert(BG_EPI_WARPS * 4096 <= STAGES * L::STAGE, "a box per warp");
+      uint8_t* const box = smem + (warp - 2) * 4096;
+      const int rows = p.M - (m0 + q * 32) < 32 ? p.M - (m0 + q * 32) : 32;
+      const long long o = (long long)(m0 + q * 32) * p.ldc + n;
+      if (p.c_type == GSB200_F32) {
+        constexpr int W = CW < 32 ? CW : 32;
+#pragma unroll
+        for (int c0 = 0; c0 < CW; c0 += W) {
+          if (n + c0 >= p.N) continue;
+          store_by_rows<uint32_t, W / 4>(box, lane, [&](int pc) {
+            const float* a = acc + c0 + 4 * pc;
+            return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+          }, static_cast<uint32_t*>(p.C) + o + c0, p.ldc, rows, p.N - n - c0);
+        }
+      } else {
+        const bool f16 = p.c_type == GSB200_F16;
+        store_by_rows<uint16_t, CW / 8>(box, lane, [&](int pc) {
+          const float* a = acc + 8 * pc;
+          return f16 ? make_uint4(pack_half2(a[0], a[1]), pack_half2(a[2], a[3]), pack_half2(a[4], a[5]), pack_half2(a[6], a[7]))
+                     : make_uint4(pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3]), pack_bf2(a[4], a[5]), pack_bf2(a[6], a[7]));
+        }, static_cast<uint16_t*>(p.C) + o, p.ldc, rows, p.N - n);
       }
     }
   }
