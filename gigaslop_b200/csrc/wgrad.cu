@@ -355,11 +355,14 @@ static bool wgrad_shape_ok(long long M, int N, int K) {
   return M >= 0 && M <= 0x7fffff00ll && N > 0 && K > 0 && N <= (1 << 24) && K <= (1 << 24) &&
          (long long)((N + 255) / 256) * ((K + WG_BK - 1) / WG_BK) <= (1 << 24);
 }
+// What goes through the workspace: parts, and sums whose rows TMA could not write to a dW of their own width (us, M = 4096, N = 4096, K = 4095, written element by
+// element by the kernel 184, so 130; M = 8300, N = 9704, K = 1001, fp16, in segments, 890 and 244).
+static bool wgrad_by_workspace(int K, int parts) { return parts > 1 || K % 4 != 0; }
 int64_t wgrad_workspace_bytes(long long M, int N, int K) {
   if (!wgrad_shape_ok(M, N, K)) return 0;
   int acc, tiles, steps, parts; long long ld, rows;
   wgrad_plan(M, N, K, acc, tiles, steps, parts, ld, rows);
-  return parts > 1 ? 4 * ld * rows * parts : 0;
+  return wgrad_by_workspace(K, parts) ? 4 * ld * rows * parts : 0;
 }
 
 template <typename T, int ACC>
@@ -408,7 +411,7 @@ int32_t launch_wgrad(const void* dy, int dt, long long lddy, const uint8_t* q, l
   if (!tmap_2d(&tm, dt == GSB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, (uint64_t)M, (uint64_t)N,
                (uint64_t)lddy, 64, WG_BM, CU_TENSOR_MAP_SWIZZLE_128B)) return GSB200_ERR_BAD_ARG;
   p.q = q; p.ldq = ldq; p.s = s; p.lds = lds; p.M = M; p.N = N; p.K = K; p.k_tiles = (K + WG_BK - 1) / WG_BK;
-  const bool cut = p.parts > 1;
+  const bool cut = wgrad_by_workspace(K, p.parts);
   p.out = cut ? static_cast<float*>(ws) : dw; p.ldo = cut ? ld : lddw; p.part_rows = cut ? rows : 0;
   // (TMA writes whole 16-byte pieces)
   p.tma_out = cut || ((reinterpret_cast<uintptr_t>(dw) & 15) == 0 && lddw % 4 == 0 && K % 4 == 0);
