@@ -50,7 +50,7 @@ struct BgSmem {
   static constexpr int SCALES = OUT + BG_EPI_WARPS * BG_OUT_BUF;          // [SC][2][BG_BM] products of the scales
   static constexpr int BAR = SCALES + SC * 2 * BG_BM * 4;
   static constexpr int BYTES = BAR + 256 + 1024;
-  static_assert(BYTES <= 227 * 1024 && (2 * STAGES + 2 * ACC) * 8 + 8 <= 256, "shared memory budget");
+  static_assert(BYTES <= 227 * 1024 && (2 * STAGES + 2 * ACC + SC) * 8 + 8 <= 256, "shared memory budget");
 };
 
 __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
@@ -105,7 +105,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + ACC;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACC);
+  uint64_t* sc_empty = acc_empty + ACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + SC);
   float* sc_smem = reinterpret_cast<float*>(smem + L::SCALES);
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -118,6 +119,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int s = 0; s < ACC; ++s) { mbar_init(&acc_full[s], 1 + 2); mbar_init(&acc_empty[s], 2 * BG_EPI_WARPS); }
+    for (int s = 0; s < SC; ++s) mbar_init(&sc_empty[s], BG_EPI_WARPS);
     abort_flag.set(0);
     fence_mbar_init();
     prefetch_tmap(&tm_a); prefetch_tmap(&tm_b); prefetch_tmap(&tm_c);
@@ -178,8 +180,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     } else if (warp >= 2) {
       // The products of the scales, ahead of the MMAs: two rows and both column halves per lane, loaded ahead.  A K
       // block's arrival completes acc_full together with the MMAs' (the one wait of the epilogue covers both), and must follow the
-      // barrier's previous phase, ACC K blocks back.  By then those MMAs were allowed to start, so the epilogue is done with the K block
-      // 2 ACC back, whose place this one takes.
+      // barrier's previous phase, ACC K blocks back.  The place that it takes in shared memory held the K block 2 ACC back.  The epilogue warps hand it back
+      // on a barrier of its own (sc_empty): the arrival that returns their stage is relaxed and orders no read of shared memory.  They do so behind the K
+      // block's multiply-adds, off the chain (us, M = 65536, N = 1536, K = 512 / N = 512, K = 2048 / N = 640, K = 512: so 71.7 / 75.1 / 45.8; right behind the
+      // read 73.3 / 75.9 / 45.0; a barrier for half of the places 73.1 / 75.2 / 44.3).
       const int r = (warp - 2) * 64 + lane;
       constexpr int FAR = 4;                                 // K blocks that are loaded ahead
       float a0[FAR], a1[FAR], b0[FAR], b1[FAR];
@@ -200,9 +204,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       bool ok = true;
       uint32_t i = 0;
       auto put = [&](int j) {
-        const uint32_t as = i % ACC;
+        const uint32_t as = i % ACC, place = i % SC;
+        if (i >= SC && !__all_sync(0xffffffffu, mbar_wait<true>(&sc_empty[place], (i / SC - 1) & 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE48 | place, budget))) { ok = false; return; }
         if (i >= ACC && !__all_sync(0xffffffffu, mbar_wait<true>(&acc_full[as], (i / ACC - 1) & 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xE40 | as, budget))) { ok = false; return; }
-        float* d = sc_smem + i % SC * 2 * BG_BM + r;
+        float* d = sc_smem + place * 2 * BG_BM + r;
         d[0] = a0[j] * b0[j]; d[32] = a1[j] * b0[j]; d[BG_BM] = a0[j] * b1[j]; d[BG_BM + 32] = a1[j] * b1[j];
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_full[as]);
@@ -266,6 +271,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             acc[32 * c + 2 * i] = r.x; acc[32 * c + 2 * i + 1] = r.y;
           }
         }
+        __syncwarp();                                        // (every lane has read its scale)
+        if (lane == 0) mbar_arrive(&sc_empty[(it - 1) % SC]);
         if (more && !there) {
           ok = stage_there();
           if (!ok) break;
