@@ -8,7 +8,7 @@
 //   its gradient from the checkpoints: du = dh g^ sigmoid(g^),  dg = dh u^ sigmoid(g^) (1 + g^ sigmoid(-g^))
 //
 // A scale that is a power of two costs E4M3, a floating-point format, no relative precision; the division is exact, so the one rounding
-// is the conversion, and a restored element is exact in fp32, in bf16, and in fp16 within its range.
+// is the conversion, and a restored element is exact in fp32, in bf16, and in fp16 within its range (the weight gradient extends that: wgrad.cu).
 //
 // All of them are bound by HBM.  A lane owns 8 consecutive elements, so a block is half a warp, and its maximum four shuffles.
 #include <cuda_bf16.h>

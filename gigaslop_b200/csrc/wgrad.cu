@@ -2,9 +2,16 @@
 //
 //   dW[n, k] (+)= sum over m of dY[m, n] x^[m, k],     x^[m, k] = s[m, k / 128] q[m, k]
 //
-// dY is 16-bit, x^ is restored on chip: E4M3 times a power of two is exact in 16 bits (fp16: inside its range), so nothing is lost
+// dY is 16-bit, x^ is restored on chip: E4M3 times a power of two is exact in 16 bits, so nothing is lost
 // against a 16-bit copy of the checkpoint that never exists in memory.  (A scale that is no power of two rounds the product to dY's
 // type.)  The reduction runs over the rows of both operands, which the tensor core reads "MN-major".
+//
+// fp16 has not the range for that, and both operands of an MMA have one type.  So x^ is restored times a power of two, and the sums are divided by
+// it, both exact.  A pass over the batch takes the rows whose scales, in these 128 columns, lie in a window of 22 powers of two: the largest become at most 2^7, 448
+// of which fit, and the smallest keep all bits of E4M3.  The window is laid about the scales of 32 rows of the part, with more room above them than below; a row
+// outside counts as zeros in the pass.  Only where there was one, other than of zeros, the scales are looked through and passes with windows above and below
+// follow.  us, fp16, without all this / with: M = 65536, N = 2048, K = 512 114.5 / 113.3, N = 512 43.0 / 40.9, M = 9001, N = 1000, K = 520 23.8 / 24.4, M = 1, N = 512,
+// K = 512 7.7 / 8.2.  (The range of all scales looked up first: 4096 x 4096 x 4096 106 / 121, a column of scales is a load per row.)
 //
 // A CTA pair (cta_group::2) computes 512 x 256 of dW (two accumulators of 128 rows in each CTA, all of its tensor memory; narrow layers
 // 256 x 256, one accumulator) over a range of rows of the batch, 64 rows per step.  A CTA holds its own rows of dW, i.e. columns of dY, and half
@@ -80,6 +87,9 @@ __device__ __forceinline__ void restore16<__nv_bfloat16>(uint4 r, float s, uint4
   lo = make_uint4(o[0], o[1], o[2], o[3]); hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+constexpr int WG_WINDOW = 22;                              // fp16: powers of two that a pass covers
+__device__ __forceinline__ int scale_exponent(float s) { return (int)(__float_as_uint(s) >> 23) & 255; }
+
 template <typename T, int ACC>
 __global__ void __launch_bounds__(WG_THREADS, 1)
 wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_out, const WgParams p) {
@@ -87,12 +97,17 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wg_smem_raw) + 1023) & ~uintptr_t(1023));
   using L = WgSmem<ACC>;
   constexpr int STAGES = L::STAGES, WG_SEG = WG_SEGMENT<T>;
+  constexpr bool WINDOWS = std::is_same<T, __half>::value;
   uint64_t* full_a = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* full_b = full_a + STAGES;
   uint64_t* empty = full_b + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  uint64_t* left_full = acc_empty + 1;                     // (fp16) left[0] is known: whether either CTA has left scales out of the first pass
+  uint64_t* more_full = left_full + 1;                     // if so, left[1] and left[2]: how many passes above and below it their rows need
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(more_full + 1);
+  int* left = reinterpret_cast<int*>(tmem_slot + 2);
+  static_assert((3 * STAGES + 4) * 8 + 8 + 12 <= 256, "room for the barriers");
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();                 // the pair's first CTA issues the MMAs; its barriers collect both CTAs' operands
@@ -102,61 +117,85 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_a[s], 1); mbar_init(&full_b[s], 2 * WG_WARPS); mbar_init(&empty[s], 1); }
-    mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS);
+    mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS); mbar_init(left_full, 2 * WG_WARPS); mbar_init(more_full, 2 * WG_WARPS);
+    left[0] = left[1] = left[2] = 0;
     abort_flag.set(0);
     fence_mbar_init();
     prefetch_tmap(&tm_dy); prefetch_tmap(&tm_out);
   }
   if (warp == 1) { tmem_alloc_pair(tmem_slot, 256 * ACC); tmem_relinquish_pair(); }
   pdl_wait();
+  float sample[2] = {0.f, 0.f};                            // scales of a row in both CTAs' columns: every warp looks at the same 32 rows of the part
+  if (WINDOWS && warp >= WG_FRONT) {
+    const long long r0 = (long long)step0 * WG_BM, r1 = (long long)step1 * WG_BM < p.M ? (long long)step1 * WG_BM : p.M;
+    const float* const f = p.s + (r0 + (r1 - r0) * lane / 32) * p.lds + (k0 >> 7);
+    sample[0] = f[0];
+    if (k0 + 128 < p.K) sample[1] = f[1];
+  }
   tc_fence_before();
   cluster_sync_all();                                      // (a __syncthreads of both CTAs) the other's barriers are initialised before anything arrives at them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const unsigned int budget = spin_budget();
+  // Passes behind the first one (-1: gave up).
+  auto left_out = [&]() { return mbar_wait_cluster(left_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF50, budget) ? left[0] : -1; };
+  auto more_passes = [&]() {
+    if constexpr (!WINDOWS) return 0;
+    const int n = left_out();
+    return n <= 0 ? n : mbar_wait_cluster(more_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF58, budget) ? left[1] + left[2] : -1;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
       int s = 0; uint32_t ph = 0;
-      for (int i = step0; i < step1; ++i) {
-        if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xF00 | s, budget)) { ok = false; break; }
-        uint8_t* st = smem + s * L::STAGE;
-        const uint32_t bar = mapa_shared(smem_u32(&full_a[s]), 0);
-        if (rank == 0) mbar_arrive_expect_tx(&full_a[s], 2 * L::A_BYTES);
+      auto feed = [&]() {
+        for (int i = step0; i < step1; ++i) {
+          if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_PRODUCER, 0xF00 | s, budget)) { ok = false; break; }
+          uint8_t* st = smem + s * L::STAGE;
+          const uint32_t bar = mapa_shared(smem_u32(&full_a[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full_a[s], 2 * L::A_BYTES);
 #pragma unroll
-        for (int j = 0; j < 2 * ACC; ++j) tma_load_2d_pair(st + j * WG_CHUNK, &tm_dy, bar, n0 + 256 * (j >> 1) + 64 * (j & 1), i * WG_BM);
-        if (++s == STAGES) { s = 0; ph ^= 1; }
-      }
-      if (!ok) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }
+          for (int j = 0; j < 2 * ACC; ++j) tma_load_2d_pair(st + j * WG_CHUNK, &tm_dy, bar, n0 + 256 * (j >> 1) + 64 * (j & 1), i * WG_BM);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      };
+      feed();
+      for (int n = ok ? more_passes() : 0; ok && n > 0; --n) feed();
+      if (!ok || abort_flag.get()) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }      // loads in flight land before the CTA exits
     }
   } else if (warp == 1 && rank == 0) {
     constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t idesc = umma_idesc(1, fmt, fmt, 256, WG_BK) | UMMA_A_MN | UMMA_B_MN;
-    int s = 0; uint32_t ph = 0;
-    for (int i = step0; i < step1; ++i) {
-      // x^ of the second CTA lies in that CTA's shared memory, and it is that SM's tensor core that reads it there.  The stores are in place when
-      // the arrival leaves the SM: each writer passes them to the async proxy and its warp arrives behind that.  (An arrival with a
-      // release to the cluster also waits for the loads in flight, 1400 clocks of each step: 184 us instead of 106 at M = 65536, N = 2048, K = 512.)
-      if (!__all_sync(0xffffffffu, mbar_wait<true>(&full_a[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF10 | s, budget)) ||
-          !__all_sync(0xffffffffu, mbar_wait<true>(&full_b[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF20 | s, budget))) break;
-      const int in_seg = (i - step0) % WG_SEG;
-      if (in_seg == 0 && i != step0 &&
-          !__all_sync(0xffffffffu, mbar_wait<true>(acc_empty, ((i - step0) / WG_SEG - 1) & 1, abort_flag, ST_TIMEOUT_MMA, 0xF60, budget))) break;
-      tc_fence_after();
-      const uint32_t st = smem_u32(smem + s * L::STAGE);
-      const uint64_t a_desc = umma_smem_desc_mn<128>(st, WG_CHUNK), b_desc = umma_smem_desc_mn<128>(st + L::A_BYTES, WG_CHUNK);
-      constexpr uint64_t step = (16 * 128) >> 4;           // K = 16: 16 rows of 128 bytes
+    bool ok = true;
+    int s = 0, segs = 0; uint32_t ph = 0;                   // segs: accumulations started
+    auto multiply = [&]() {
+      for (int i = step0; i < step1; ++i) {
+        // x^ of the second CTA lies in that CTA's shared memory, and it is that SM's tensor core that reads it there.  The stores are in place when
+        // the arrival leaves the SM: each writer passes them to the async proxy and its warp arrives behind that.  (An arrival with a
+        // release to the cluster also waits for the loads in flight, 1400 clocks of each step: 184 us instead of 106 at M = 65536, N = 2048, K = 512.)
+        if (!__all_sync(0xffffffffu, mbar_wait<true>(&full_a[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF10 | s, budget)) ||
+            !__all_sync(0xffffffffu, mbar_wait<true>(&full_b[s], ph, abort_flag, ST_TIMEOUT_MMA, 0xF20 | s, budget))) { ok = false; break; }
+        const int in_seg = (i - step0) % WG_SEG;
+        if (in_seg == 0 && segs++ != 0 &&                      // the accumulators' previous sums are out
+            !__all_sync(0xffffffffu, mbar_wait<true>(acc_empty, segs & 1, abort_flag, ST_TIMEOUT_MMA, 0xF60, budget))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem + s * L::STAGE);
+        const uint64_t a_desc = umma_smem_desc_mn<128>(st, WG_CHUNK), b_desc = umma_smem_desc_mn<128>(st + L::A_BYTES, WG_CHUNK);
+        constexpr uint64_t step = (16 * 128) >> 4;           // K = 16: 16 rows of 128 bytes
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k) {
 #pragma unroll
-        for (int j = 0; j < ACC; ++j)
-          umma_f16_pair_elect(tmem_base + 256 * j, a_desc + (j * 2 * WG_CHUNK >> 4) + step * k, b_desc + step * k, idesc, in_seg != 0 || k != 0);
+          for (int j = 0; j < ACC; ++j)
+            umma_f16_pair_elect(tmem_base + 256 * j, a_desc + (j * 2 * WG_CHUNK >> 4) + step * k, b_desc + step * k, idesc, in_seg != 0 || k != 0);
+        }
+        umma_commit_pair_both_elect(&empty[s]);
+        if (in_seg == WG_SEG - 1 || i + 1 == step1) umma_commit_pair_both_elect(acc_full);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
       }
-      umma_commit_pair_both_elect(&empty[s]);
-      if (in_seg == WG_SEG - 1 || i + 1 == step1) umma_commit_pair_both_elect(acc_full);
-      if (++s == STAGES) { s = 0; ph ^= 1; }
-    }
+    };
+    multiply();
+    for (int n = ok ? __shfl_sync(0xffffffffu, more_passes(), 0) : 0; ok && n > 0; --n) multiply();
   } else if (warp >= WG_FRONT) {
     // Thread: 16 columns of x^ (two 16-byte pieces of a row of the tile), rows r and r + 32 of the step, loaded WG_AHEAD steps ahead (a step is
     // shorter than a read of HBM).
@@ -164,8 +203,13 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
     const int k = k0 + 128 * rank + 16 * c;
     const int have = p.K - k;                              // columns left from k on
     const long long dq = 32 * p.ldq, ds = 32 * p.lds;      // (to the thread's other row)
-    const uint8_t* qp = p.q + ((long long)step0 * WG_BM + r) * p.ldq + (have > 0 ? k : 0);
-    const float* sp = p.s + ((long long)step0 * WG_BM + r) * p.lds + (have > 0 ? k >> 7 : 0);
+    const uint8_t* qp;
+    const float* sp;
+    auto rewind = [&]() {
+      qp = p.q + ((long long)step0 * WG_BM + r) * p.ldq + (have > 0 ? k : 0);
+      sp = p.s + ((long long)step0 * WG_BM + r) * p.lds + (have > 0 ? k >> 7 : 0);
+    };
+    rewind();
     uint4 raws[WG_AHEAD][2];
     float scs[WG_AHEAD][2];
     auto fetch = [&](int i, uint4 (&raw)[2], float (&sc)[2]) {
@@ -203,9 +247,31 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
     };
 #pragma unroll
     for (int a = 0; a < WG_AHEAD; ++a) fetch(step0 + a, raws[a], scs[a]);
+    int tops[2] = {0, 0};                                  // greatest exponents of the pass, in both CTAs' columns of x^
+    if constexpr (WINDOWS) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = scale_exponent(sample[i]);
+        const bool counts = sample[i] != 0.f && e != 255;
+        const int h = __reduce_max_sync(0xffffffffu, counts ? e : -1), l = __reduce_min_sync(0xffffffffu, counts ? e : 256);
+        const int room = WG_WINDOW - 1 - (h - l);
+        tops[i] = h < l ? 130 : h + (room > 0 ? room * 2 / 3 : 0);
+      }
+    }
     const uint32_t arrive_b = mapa_shared(smem_u32(full_b), 0);
     const int swap = (c >> 2) & 1, pc = 2 * (c & 3);       // half of the lanes store their second piece first: no bank conflicts
     bool ok = true;
+    int top = 0;                                           // of this CTA's columns
+    float up = 1.f;                                        // the factor on them
+    auto factor_exponent = [](int e) { return max(min(260 - e, 253), 1); };        // 2^(133 - e): scales of exponent e become 2^6 .. 2^7
+    uint32_t outside = 0;                                  // bits of the scales outside the pass
+    // The factor of a row.  (Without a branch: the loads ahead wait at one, M = 9001, N = 1000, K = 520 26.1 us.  Infinite and NaN scales have a pass of their own.)
+    auto factor = [&](float sc) {
+      if constexpr (!WINDOWS) return sc;
+      const bool in = (unsigned)(top - scale_exponent(sc)) < (unsigned)WG_WINDOW;
+      outside |= in ? 0u : __float_as_uint(sc) & 0x7fffffffu;
+      return in ? sc * up : 0.f;
+    };
     // Segment `seg` of the sums to dW.  Warp: lane quarter; of two accumulators one per four warps, of one its column halves.
     auto drain = [&](int seg) {
       const int q = warp & 3, half = (warp - WG_FRONT) >> 2;
@@ -224,6 +290,11 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
         __syncwarp();
         tmem_ld_32x32b_x32(t + c0, v);
         tmem_ld_wait(v);
+        if constexpr (WINDOWS) {
+          const float down = __uint_as_float((uint32_t)(254 - factor_exponent(cb + c0 < 128 ? tops[0] : tops[1])) << 23);
+#pragma unroll
+          for (int b = 0; b < 32; ++b) v[b] = __float_as_uint(__uint_as_float(v[b]) * down);
+        }
         if (p.tma_out) {
           if (lane == 0) tma_store_wait_read<0>();         // the previous box has left the buffer
           __syncwarp();
@@ -248,49 +319,114 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
     };
     const uint32_t drained = mapa_shared(smem_u32(acc_empty), 0);
     static_assert(WG_SEG % WG_AHEAD == 0 && WG_AHEAD <= STAGES, "a segment is whole rounds of the loop below, and a round fits the ring");
-    int s = 0; uint32_t ph = 0;
-    for (int i0 = step0; ok && i0 < step1; i0 += WG_AHEAD) {
-      // (the next segment's first steps are in shared memory before: its MMAs start as soon as the sums are out)
-      if (i0 - step0 > WG_SEG && (i0 - step0) % WG_SEG == WG_AHEAD) {
-        drain((i0 - step0) / WG_SEG - 1);
-        if (!ok) break;
+    int s = 0, seg0 = 0; uint32_t ph = 0;                  // seg0: segments before the pass
+    auto run_pass = [&](auto first_pass) {
+      constexpr bool FIRST = decltype(first_pass)::value;
+      if constexpr (WINDOWS) {
+        top = rank == 0 ? tops[0] : tops[1];
+        up = __uint_as_float((uint32_t)factor_exponent(top) << 23);
+        if constexpr (!FIRST) {
+          rewind();
+#pragma unroll
+          for (int a = 0; a < WG_AHEAD; ++a) fetch(step0 + a, raws[a], scs[a]);
+          tc_fence_before();                               // the pass before has read its last sums
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(drained);
+        }
+      }
+      for (int i0 = step0; ok && i0 < step1; i0 += WG_AHEAD) {
+        // (the next segment's first steps are in shared memory before: its MMAs start as soon as the sums are out)
+        if (i0 - step0 > WG_SEG && (i0 - step0) % WG_SEG == WG_AHEAD) {
+          drain(seg0 + (i0 - step0) / WG_SEG - 1);
+          if (!ok) break;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(drained);
+        }
+#pragma unroll
+        for (int a = 0; a < WG_AHEAD; ++a) {
+          const int i = i0 + a;
+          if (i >= step1) break;
+          uint4 lo[2], hi[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) restore16<T>(raws[a][j], factor(scs[a][j]), lo[j], hi[j]);
+          fetch(i + WG_AHEAD, raws[a], scs[a]);
+          ok = __all_sync(0xffffffffu, mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF30 | s, budget));
+          if (!ok) break;
+          uint8_t* tile_b = smem + s * L::STAGE + L::A_BYTES + (c >> 2) * WG_CHUNK;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int row = r + 32 * j;
+            uint8_t* line = tile_b + row * 128;
+            *reinterpret_cast<uint4*>(line + (((pc + swap) ^ (row & 7)) << 4)) = swap ? hi[j] : lo[j];
+            *reinterpret_cast<uint4*>(line + (((pc + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo[j] : hi[j];
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(arrive_b + 8 * s);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      }
+      // (the last segment; and the one before it, if this one was too short to come to that above)
+      const int last = (step1 - step0 - 1) / WG_SEG;
+      if (ok && last > 0 && step1 - step0 - last * WG_SEG <= WG_AHEAD) {
+        drain(seg0 + last - 1);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(drained);
+        if (ok && lane == 0) mbar_arrive_remote(drained);
       }
+      if constexpr (WINDOWS && FIRST) {
+        const bool any = __any_sync(0xffffffffu, outside != 0u);
+        if (lane == 0) {
 #pragma unroll
-      for (int a = 0; a < WG_AHEAD; ++a) {
-        const int i = i0 + a;
-        if (i >= step1) break;
-        uint4 lo[2], hi[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) restore16<T>(raws[a][j], scs[a][j], lo[j], hi[j]);
-        fetch(i + WG_AHEAD, raws[a], scs[a]);
-        ok = __all_sync(0xffffffffu, mbar_wait<true>(&empty[s], ph ^ 1, abort_flag, ST_TIMEOUT_EPILOGUE, 0xF30 | s, budget));
-        if (!ok) break;
-        uint8_t* tile_b = smem + s * L::STAGE + L::A_BYTES + (c >> 2) * WG_CHUNK;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = r + 32 * j;
-          uint8_t* line = tile_b + row * 128;
-          *reinterpret_cast<uint4*>(line + (((pc + swap) ^ (row & 7)) << 4)) = swap ? hi[j] : lo[j];
-          *reinterpret_cast<uint4*>(line + (((pc + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo[j] : hi[j];
+          for (uint32_t to = 0; to < 2; ++to) {
+            const uint32_t bar = mapa_shared(smem_u32(left_full), to);
+            if (any) {
+              red_max_cluster(mapa_shared(smem_u32(left), to), 1);
+              mbar_arrive_remote_release(bar);
+            } else {
+              mbar_arrive_remote_relaxed(bar);             // (nothing to order, and a release takes a microsecond)
+            }
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(arrive_b + 8 * s);
-        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+      if (ok) drain(seg0 + last);
+      seg0 += last + 1;
+    };
+    run_pass(std::true_type{});
+    if constexpr (WINDOWS) {
+      if (ok && __shfl_sync(0xffffffffu, left_out(), 0) > 0) {
+        int above = 0, below = 0;                          // (infinite and NaN scales have the greatest exponent, 255)
+        rewind();
+        for (int i = step0; i < step1; ++i) {
+          fetch(i, raws[0], scs[0]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 q = raws[0][j];
+            const int e = scale_exponent(scs[0][j]);
+            if (scs[0][j] == 0.f || (e != 255 && ((q.x | q.y | q.z | q.w) & 0x7f7f7f7fu) == 0u)) continue;
+            above = max(above, (e - top + WG_WINDOW - 1) / WG_WINDOW);
+            below = max(below, (top - e) / WG_WINDOW);
+          }
+        }
+        above = __reduce_max_sync(0xffffffffu, above);
+        below = __reduce_max_sync(0xffffffffu, below);
+        if (lane == 0) {
+          for (uint32_t to = 0; to < 2; ++to) {
+            red_max_cluster(mapa_shared(smem_u32(left + 1), to), above);
+            red_max_cluster(mapa_shared(smem_u32(left + 2), to), below);
+            mbar_arrive_remote_release(mapa_shared(smem_u32(more_full), to));
+          }
+        }
+        const int n = __shfl_sync(0xffffffffu, more_passes(), 0), up_to = n > 0 ? left[1] : 0;
+        for (int i = 1; ok && i <= n; ++i) {               // upwards, then from the first one downwards
+          const int by = (i <= up_to ? 1 : i == up_to + 1 ? -1 - up_to : -1) * WG_WINDOW;
+          tops[0] += by;
+          tops[1] += by;
+          run_pass(std::false_type{});
+        }
       }
     }
-    // (the last segment; and the one before it, if this one was too short to come to that above)
-    const int last = (step1 - step0 - 1) / WG_SEG;
-    if (ok && last > 0 && step1 - step0 - last * WG_SEG <= WG_AHEAD) {
-      drain(last - 1);
-      tc_fence_before();
-      __syncwarp();
-      if (ok && lane == 0) mbar_arrive_remote(drained);
-    }
-    if (ok) drain(last);
     if (lane == 0) tma_store_wait_all<0>();
   }
   tc_fence_before();

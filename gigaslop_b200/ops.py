@@ -635,7 +635,8 @@ def _checked_gemm_fp8_block(A, B, scale_a, scale_b, out, dtype, b_transposed):
 
 def gemm_fp8_block_wgrad(dy, q, scale, out=None, accumulate=False):
     """Weight gradient ``dY^T . X`` [N,K] fp32 from ``dy`` [M,N] fp16/bf16 and the block-scaled 8-bit checkpoint ``q`` [M,K],
-    ``scale`` [M, ceil(K/128)] of the layer's input.  ``accumulate`` adds to ``out``.  Rows of ``dy`` on 16-byte boundaries."""
+    ``scale`` [M, ceil(K/128)] of the layer's input.  ``accumulate`` adds to ``out``.  Rows of ``dy`` on 16-byte boundaries.  The
+    checkpoint is restored to ``dy``'s significand, without loss for scales that are powers of two, whatever their size."""
     n = _lib.native
     if n is not None:
         r = n.block_wgrad(dy, q, scale, out, accumulate)
