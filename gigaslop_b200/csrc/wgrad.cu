@@ -34,11 +34,12 @@ constexpr int WG_BK = 256, WG_BM = 64;                     // columns of x^ (a p
 constexpr int WG_WARPS = 8, WG_FRONT = 4, WG_THREADS = 32 * (WG_WARPS + WG_FRONT);
 constexpr int WG_CHUNK = WG_BM * 128;                      // a 64-column chunk of an operand tile: 64 rows of 128 bytes
 // Steps of 64 rows that the tensor core sums by itself.  Its fp32 additions truncate, which takes a little off a sum with each, fp16's longer products
-// more than bf16's: M = 65536, N = 2048, K = 512, bf16 comes out 3.2e-6 off (2-norm) from parts of 114 steps, 1.35e-6 from segments of 64, 9.8e-7 from 48,
-// 6e-7 from 32 (plain fp32 sums: 2e-7); M = 9001, fp16 1.2e-6 from 24.  It grows with the steps, so long parts are added to dW in segments, in fp32 as
-// the parts are.  Each costs 7 us, the time of 256 KiB per CTA through L2 (without 105 us, segments of 64 114, of 32 130; written by the threads instead of
-// by TMA 120 and 167).
-template <typename T> constexpr int WG_SEGMENT = std::is_same<T, __half>::value ? 64 : 128;
+// more than bf16's, so what it has summed is added to dW in segments, in fp32 as the parts are.  They are as long as keeps the error of random terms
+// below 2^-19 in the 2-norm, whatever the batch.  Error / us (each segment costs 7, the time of 256 KiB per CTA through L2; written by the threads instead of by
+// TMA 15 to 30) at M = 65536, N = 2048, K = 512, segments of 32, 48, 64, 128 steps: bf16 6.1e-7 / 126, 9.9e-7 / 118, 1.4e-6 / 112, 3.2e-6 (unsegmented) / 103; fp16
+// 1.7e-6 / 126, 2.6e-6 / 119, 3.5e-6 / 112.  M = 65536, N = 4096, K = 4096: bf16 6.5e-7, 1.1e-6, 1.5e-6, 3.7e-6, fp16 1.8e-6, 2.8e-6, 3.9e-6; plain fp32
+// products 1.5e-6 and 3.0e-6 (2e-7 where the batch is short).
+template <typename T> constexpr int WG_SEGMENT = std::is_same<T, __half>::value ? 32 : 64;
 constexpr int WG_AHEAD = 4;                                // steps of x^ in flight to the registers
 constexpr int WG_B_BYTES = 2 * WG_CHUNK;                   // a CTA's 128 columns of x^
 template <int ACC>                                         // accumulators (128 rows of dW per CTA each)

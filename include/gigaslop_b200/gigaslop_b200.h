@@ -272,7 +272,9 @@ int32_t gsb200_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* scale_
  * accumulate != 0 adds to what dW holds (gradient accumulation).  dY fp16 or bf16 [M,N], q / scale as the forward pass's quantiser left
  * them [M,K].  q * scale is rounded to dY's significand on its way to the tensor cores: exact for scales that are powers of two, 2^-124 to 2^119
  * (fp16 has its range extended by exact factors; scales of a column block that are more than 2^21 apart cost it another pass over the batch);
- * others to 8 bits, or to 11 (fp16) and 2^-10 of the scale.  The order of the sums depends on the sizes alone.  M = 0 gives zeros (or leaves dW as it is).
+ * others to 8 bits, or to 11 (fp16) and 2^-10 of the scale.  The tensor cores' sums truncate and are therefore added up in
+ * fp32 every 4096 rows (fp16: 2048), which keeps dW within 2^-19 of the exact one (2-norm, terms of random sign).  The order of the sums depends on the
+ * sizes alone.  M = 0 gives zeros (or leaves dW as it is).
  * N and K up to 2^24 (2^24 tiles of 256 x 256).  A CTA ends with its tile: no gsb200_set_sm_limit.
  * workspace: gsb200_gemm_fp8_block_wgrad_workspace_bytes(M, N, K) bytes (may be 0), 32-byte aligned; calls that may overlap
  * need one each. */

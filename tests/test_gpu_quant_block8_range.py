@@ -140,3 +140,18 @@ def test_down_projection_gradient_of_small_activations():
     assert float(mag.min()) > 0 and bool(((dw.double() - want).abs() <= bound(want, mag, m + 160)).all())
     exact = dy.double().t() @ block8.swiglu(gate.double(), up.double())
     assert float((dw.double() - exact).norm() / exact.norm()) <= 2.0 ** -4      # (each element of h is off by 2^-4 at most)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(65536, 2048, 512), (65536, 512, 512), (65536, 1536, 2048), (65536, 200, 1024), (8192, 4096, 4096), (9000, 256, 9472), (3000, 512, 512)])
+def test_wgrad_truncation_stays_small(m, n, k, dt):
+    """The header's bound on the sums: 2^-19 of the 2-norm.  (The tensor core's own sums of 7300 rows are 1.7 times as far off, with every shortened sum
+    nearer to zero.)"""
+    g = need_lib()
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    q, s = g.fp8_block_quantize(torch.randn(m, k, generator=gen, device="cuda").to(dt))
+    dy = gradient(gen, m, n, dt)
+    want = dy.double().t() @ block8.values(q, s)
+    dw = g.gemm_fp8_block_wgrad(dy, q, s)
+    assert float((dw.double() - want).norm() / want.norm()) <= 2.0 ** -19
+    assert g.device_status()[0] == 0
