@@ -285,7 +285,7 @@ int32_t gsb200_gemm_fp8_block_wgrad(const void* dY, int32_t dy_dtype, int64_t ld
 
 /* SwiGLU into the format, with checkpoints: h = gate * sigmoid(gate) * up in fp32, quantised from there (the down-projection's operand), and
  * gate and up quantised for the backward pass.  gate, up [M,F] of one type; the three outputs share their row strides.
- * The sigmoid is taken in fp32: below gate = -87 it may be 0.
+ * The sigmoid is taken in fp32; of 16-bit gates below -87 it may be 0.
  * The gradient reads the checkpoints (any scales): with s = sigmoid(gate), dup = dh * gate * s, dgate = dh * up * s * (1 + gate * (1 - s)), in
  * dh's type.  dgate_q .. dup_s (all four or none): the two gradients quantised as well, from their rounded values, for the input gradient's
  * product. */

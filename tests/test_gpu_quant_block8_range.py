@@ -127,6 +127,28 @@ def test_wgrad_of_a_scale_that_is_no_number(dt):
     assert bool((err <= bound(want, mag, m + 170))[:, ~bad].all())
 
 
+def test_swiglu_gradient_in_fp32_down_to_the_last_exponential():
+    """Gates to -88.7, where e^-g leaves fp32.  dup = dh g sigmoid(g): the exponential within 2 ulp (2^-22), the reciprocal within one (2^-23), and a sum and
+    three products off by 2^-24 each, are 2^-22 (1 + 1/2 + 4/4) = 1.25 2^-21 in all; dgate has a difference, a multiply-add and a product more, and as much of its terms'
+    magnitudes each at most."""
+    g = need_lib()
+    gate = torch.cat([torch.linspace(-88.7, -87.0, 200), torch.linspace(-87, 60, 312)]).cuda().view(4, 128)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    # (a gate per block of its own scale is not needed: a scale of g / 256 and the code of 256 give any fp32 gate, in blocks of one value)
+    codes_, ones = torch.full((512, 128), 0x78, dtype=torch.uint8, device="cuda").view(F8), torch.full((512, 128), 0x38, dtype=torch.uint8, device="cuda").view(F8)
+    gs = (gate.view(-1, 1) / 256).contiguous()
+    us = torch.rand(512, 1, generator=gen, device="cuda") + 0.5
+    dh = torch.randn(512, 128, generator=gen, device="cuda")
+    dg, du = g.swiglu_fp8_block_bwd(dh, codes_, gs, ones, us)
+    gv, uv = block8.values(codes_, gs), block8.values(ones, us)
+    wg, wu = block8.swiglu_bwd(dh.double(), gv, uv)
+    tiny = 2.0 ** -140                                     # (half of fp32's least step, 2^-149, times |g|, dh and u)
+    assert bool(((du.double() - wu).abs() <= 1.25 * 2.0 ** -21 * wu.abs() + tiny).all())
+    sig = torch.sigmoid(gv)
+    mag = (dh.double() * uv * sig).abs() * (1 + (gv * (1 - sig)).abs())
+    assert bool(((dg.double() - wg).abs() <= 4 * 1.25 * 2.0 ** -21 * mag + tiny).all())
+
+
 def test_down_projection_gradient_of_small_activations():
     """SwiGLU of values about 1e-4: h is about 5e-9, its checkpoint's scales about 2^-34, far below what fp16 itself holds."""
     g = need_lib()
