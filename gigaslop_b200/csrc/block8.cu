@@ -26,15 +26,6 @@ constexpr int B8_WARPS = 4;                   // (eight: the same or up to 4 % s
 template <typename T, int V> constexpr int b8_resident(bool quant = false) { return sizeof(T) == 2 && V == 2 && !quant ? 10 : 1; }
 
 // ---- 8 consecutive elements ------------------------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-
 template <typename T> struct Raw8 { uint4 w[sizeof(T) / 2]; };      // as loaded
 
 __device__ __forceinline__ float2 pair_f32(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
