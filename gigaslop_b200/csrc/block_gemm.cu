@@ -16,9 +16,11 @@
 //   warp 1      MMA issue (first CTA of the pair; converged, one elected lane)
 //   warps 2, 3  products of the scales, loaded four K blocks ahead, through shared memory
 //   warps 4..11 epilogue: lane quarter e % 4, column half e / 4
-// What bounds it is the round trip of a stage, two of which are all that tensor memory holds: MMAs (512 clocks and about 230 until the last
-// one shows), the epilogue's wake-up, four reads of 32 columns (300), the return to the MMA warp (230): about 1700 clocks for two
-// K blocks, 850 each where the MMAs alone take 512.  Everything that can leave that chain has left it: the scales (their address arithmetic,
+// A K block takes about 850 clocks where its MMAs take 512.  The round trip of a stage, two of which are all that tensor memory holds, accounts for that: MMAs
+// (512 clocks and about 230 until the last one shows), the epilogue's wake-up, four reads of 32 columns (300), the return to the MMA warp (230), 1700
+// clocks for two K blocks.  But it is not shown to be the only bound: tiles of 128 columns have four stages and half the MMAs, and still take some 600 clocks a K
+// block (0.69 of a wide tile's time, below), in which a CTA loads the same 40 bytes a clock; the operands' feed or a fixed cost per K block in the epilogue would explain
+// both.  Out of the stage's chain are the scales (their address arithmetic,
 // loads and products), the wait for the operands (before that for the stage), the multiply-adds of a chunk (behind the read of the next one,
 // the last ones behind the release).  us, M = 65536, N = 1536, K = 512 / N = 512, K = 2048: single CTAs with 256 columns that load their own scales
 // 91 / 80; pairs 95 / 80; scales through shared memory 78 / 76; two staging boxes per warp instead of one 72 / 74, filled before one fence 70 / 72.

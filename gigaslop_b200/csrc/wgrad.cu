@@ -471,8 +471,8 @@ __global__ void wgrad_reduce_kernel(const float* ws, long long ld, long long par
 }
 
 // Accumulators per CTA, tiles, and the parts the batch is cut into: what fills the SMs with pairs, at least four steps each.  Two accumulators use
-// the restored elements twice, but take half as many pairs for the same tiles and longer to write (us, K = 512, one / two accumulators: N = 2048 M = 333
-// 10.1 / 13.9, 3000 18.8 / 22.5, 9001 30.0 / 29.4, 65536 137 / 104; N = 512 M = 9001 16.8 / 22.5, 65536 43.6 / 42.1): two from 14 steps a part.  A function of the
+// the restored elements twice, but take half as many pairs for the same tiles and longer to write (us, K = 512, bf16, one / two accumulators: N = 2048
+// M = 333 10.2 / 13.4, 3000 17.6 / 19.6, 9001 31.0 / 28.9, 65536 188 / 113; N = 512 M = 9001 15.9 / 19.5, 65536 54.4 / 43.0): two from 14 steps a part.  A function of the
 // sizes alone: a workspace asked for before a device is chosen fits, and the sums have the same order everywhere.
 constexpr int WG_FILL = 74;
 static void wgrad_plan(long long M, int N, int K, int& acc, int& tiles, int& steps, int& parts, long long& ld, long long& part_rows) {
@@ -493,7 +493,7 @@ static bool wgrad_shape_ok(long long M, int N, int K) {
          (long long)((N + 255) / 256) * ((K + WG_BK - 1) / WG_BK) <= (1 << 24);
 }
 // What goes through the workspace: parts, and sums whose rows TMA could not write to a dW of their own width (us, M = 4096, N = 4096, K = 4095, written element by
-// element by the kernel 184, so 130; M = 8300, N = 9704, K = 1001, fp16, in segments, 890 and 244).
+// element by the kernel 184, so 130; M = 8300, N = 9704, K = 1001, fp16, in segments, 890 and 253).
 static bool wgrad_by_workspace(int K, int parts) { return parts > 1 || K % 4 != 0; }
 int64_t wgrad_workspace_bytes(long long M, int N, int K) {
   if (!wgrad_shape_ok(M, N, K)) return 0;

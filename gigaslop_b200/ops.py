@@ -491,6 +491,8 @@ def _checked_dual_gemm_mxfp8_silu(A, sfa_tiled, B_gate, B_up, sfb_gate_tiled, sf
 
 
 # ---- block-scaled FP8: one fp32 scale per 128 elements of a row, or per 128 x 128 tile ---------------------------------
+# The backward operators are calls of their own: as everywhere in this package, autograd sees none of it, and results are detached whatever their inputs
+# require.
 BLOCK = 128
 _BLOCK_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
@@ -604,7 +606,8 @@ def _checked_fp8_block_dequantize(q, scale, rows, dtype, out):
 def gemm_fp8_block(A, B, scale_a, scale_b, out=None, dtype=torch.float16, b_transposed=False):
     """``A[M,K] . B[N,K]^T`` over block-scaled FP8 operands -> fp16, bf16 or fp32: ``scale_a`` [M, ceil(K/128)], ``scale_b``
     [ceil(N/128), ceil(K/128)].  ``b_transposed``: B is [K,N] with scales [ceil(K/128), ceil(N/128)], which is the input gradient
-    ``dY . W`` with the weight as the forward pass has it.  Sums and scales in fp32, one rounding."""
+    ``dY . W`` with the weight as the forward pass has it.  Sums and scales in fp32, one rounding: a product of two scales has to be a
+    normal fp32 number, or 0."""
     n = _lib.native
     if n is not None:
         r = n.block_gemm(A, B, scale_a, scale_b, out, _BLOCK_DT.get(dtype, -1), b_transposed)
