@@ -104,10 +104,10 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
   uint64_t* empty = full_b + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 1;
-  uint64_t* left_full = acc_empty + 1;                     // (fp16) left[0] is known: whether either CTA has left scales out of the first pass
-  uint64_t* more_full = left_full + 1;                     // if so, left[1] and left[2]: how many passes above and below it their rows need
+  uint64_t* missed_full = acc_empty + 1;                   // (fp16) missed[0] is known: whether either CTA has left scales out of the first pass
+  uint64_t* more_full = missed_full + 1;                   // if so, missed[1] and missed[2]: how many passes above and below it their rows need
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(more_full + 1);
-  int* left = reinterpret_cast<int*>(tmem_slot + 2);
+  int* missed = reinterpret_cast<int*>(tmem_slot + 2);
   static_assert((3 * STAGES + 4) * 8 + 8 + 12 <= 256, "room for the barriers");
   const AbortFlag abort_flag{smem_u32(tmem_slot + 1)};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -118,8 +118,8 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_a[s], 1); mbar_init(&full_b[s], 2 * WG_WARPS); mbar_init(&empty[s], 1); }
-    mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS); mbar_init(left_full, 2 * WG_WARPS); mbar_init(more_full, 2 * WG_WARPS);
-    left[0] = left[1] = left[2] = 0;
+    mbar_init(acc_full, 1); mbar_init(acc_empty, 2 * WG_WARPS); mbar_init(missed_full, 2 * WG_WARPS); mbar_init(more_full, 2 * WG_WARPS);
+    missed[0] = missed[1] = missed[2] = 0;
     abort_flag.set(0);
     fence_mbar_init();
     prefetch_tmap(&tm_dy); prefetch_tmap(&tm_out);
@@ -139,11 +139,11 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
   const uint32_t tmem_base = *tmem_slot;
   const unsigned int budget = spin_budget();
   // Passes behind the first one (-1: gave up).
-  auto left_out = [&]() { return mbar_wait_cluster(left_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF50, budget) ? left[0] : -1; };
+  auto missed_any = [&]() { return mbar_wait_cluster(missed_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF50, budget) ? missed[0] : -1; };
   auto more_passes = [&]() {
     if constexpr (!WINDOWS) return 0;
-    const int n = left_out();
-    return n <= 0 ? n : mbar_wait_cluster(more_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF58, budget) ? left[1] + left[2] : -1;
+    const int n = missed_any();
+    return n <= 0 ? n : mbar_wait_cluster(more_full, 0, abort_flag, ST_TIMEOUT_PRODUCER, 0xF58, budget) ? missed[1] + missed[2] : -1;
   };
 
   if (warp == 0) {
@@ -381,9 +381,9 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
         if (lane == 0) {
 #pragma unroll
           for (uint32_t to = 0; to < 2; ++to) {
-            const uint32_t bar = mapa_shared(smem_u32(left_full), to);
+            const uint32_t bar = mapa_shared(smem_u32(missed_full), to);
             if (any) {
-              red_max_cluster(mapa_shared(smem_u32(left), to), 1);
+              red_max_cluster(mapa_shared(smem_u32(missed), to), 1);
               mbar_arrive_remote_release(bar);
             } else {
               mbar_arrive_remote_relaxed(bar);             // (nothing to order, and a release takes a microsecond)
@@ -396,7 +396,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
     };
     run_pass(std::true_type{});
     if constexpr (WINDOWS) {
-      if (ok && __shfl_sync(0xffffffffu, left_out(), 0) > 0) {
+      if (ok && __shfl_sync(0xffffffffu, missed_any(), 0) > 0) {
         int above = 0, below = 0;                          // (infinite and NaN scales have the greatest exponent, 255)
         rewind();
         for (int i = step0; i < step1; ++i) {
@@ -414,12 +414,12 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
         below = __reduce_max_sync(0xffffffffu, below);
         if (lane == 0) {
           for (uint32_t to = 0; to < 2; ++to) {
-            red_max_cluster(mapa_shared(smem_u32(left + 1), to), above);
-            red_max_cluster(mapa_shared(smem_u32(left + 2), to), below);
+            red_max_cluster(mapa_shared(smem_u32(missed + 1), to), above);
+            red_max_cluster(mapa_shared(smem_u32(missed + 2), to), below);
             mbar_arrive_remote_release(mapa_shared(smem_u32(more_full), to));
           }
         }
-        const int n = __shfl_sync(0xffffffffu, more_passes(), 0), up_to = n > 0 ? left[1] : 0;
+        const int n = __shfl_sync(0xffffffffu, more_passes(), 0), up_to = n > 0 ? missed[1] : 0;
         for (int i = 1; ok && i <= n; ++i) {               // upwards, then from the first one downwards
           const int by = (i <= up_to ? 1 : i == up_to + 1 ? -1 - up_to : -1) * WG_WINDOW;
           tops[0] += by;

@@ -103,6 +103,37 @@ def test_wgrad_of_scales_that_change_along_the_batch(ts, m, n, k, dt):
     assert g.device_status()[0] == 0
 
 
+def test_wgrad_passes_from_a_graph_and_on_two_streams():
+    """How many passes a call takes is for the device to find out: a captured call replayed over scales that need one, two and six, and calls that
+    need different numbers side by side, give the bytes of calls by themselves."""
+    g = need_lib()
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    m, n, k = 5000, 520, 300
+    q, dy = codes(gen, m, k), gradient(gen, m, n, torch.float16)
+    row = torch.arange(m, device="cuda")[:, None] * torch.ones(1, 3, device="cuda")
+    sets = [torch.exp2((row % 5) - 9), torch.exp2(30 * (row // 64 % 2) - 20), torch.exp2(100 - 25 * (row // 700))]
+    want = [g.gemm_fp8_block_wgrad(dy, q, s) for s in sets]
+    s = sets[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = g.gemm_fp8_block_wgrad(dy, q, s)
+    for i in (0, 1, 2, 0, 2):
+        s.copy_(sets[i])
+        graph.replay()
+        assert torch.equal(out, want[i])
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(g.gemm_fp8_block_wgrad(dy, q, x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i % 3]) for i, a in enumerate(got))
+    assert g.device_status()[0] == 0
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_wgrad_of_a_scale_that_is_no_number(dt):
     """An infinite or NaN scale, and a NaN element in a row of another pass, reach their own columns and no other; a scale of zero adds nothing."""
