@@ -9,9 +9,9 @@
 // fp16 has not the range for that, and both operands of an MMA have one type.  So x^ is restored times a power of two, and the sums are divided by
 // it, both exact.  A pass over the batch takes the rows whose scales, in these 128 columns, lie in a window of 22 powers of two: the largest become at most 2^7, 448
 // of which fit, and the smallest keep all bits of E4M3.  The window is laid about the scales of 32 rows of the part, with more room above them than below; a row
-// outside counts as zeros in the pass.  Only where there was one, other than of zeros, the scales are looked through and passes with windows above and below
-// follow.  us, fp16, without all this / with: M = 65536, N = 2048, K = 512 114.5 / 113.3, N = 512 43.0 / 40.9, M = 9001, N = 1000, K = 520 23.8 / 24.4, M = 1, N = 512,
-// K = 512 7.7 / 8.2.  (The range of all scales looked up first: 4096 x 4096 x 4096 106 / 121, a column of scales is a load per row.)
+// outside counts as zeros in the pass.  Where there was one, the scales are looked through, and passes with windows above and below follow as far as rows that are
+// not all zeros need them.  us, fp16, without all this / with: M = 65536, N = 2048, K = 512 114.5 / 113.3, N = 512 43.0 / 40.9, M = 9001, N = 1000, K = 520 23.8 / 24.4 (one more window
+// looked for and passed 68, five more 139), M = 1, N = 512, K = 512 7.7 / 8.2.  (The range of all scales looked up first: 4096 x 4096 x 4096 106 / 121, a column of scales is a load per row.)
 //
 // A CTA pair (cta_group::2) computes 512 x 256 of dW (two accumulators of 128 rows in each CTA, all of its tensor memory; narrow layers
 // 256 x 256, one accumulator) over a range of rows of the batch, 64 rows per step.  A CTA holds its own rows of dW, i.e. columns of dY, and half
@@ -399,15 +399,19 @@ wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ 
       if (ok && __shfl_sync(0xffffffffu, missed_any(), 0) > 0) {
         int above = 0, below = 0;                          // (infinite and NaN scales have the greatest exponent, 255)
         rewind();
-        for (int i = step0; i < step1; ++i) {
-          fetch(i, raws[0], scs[0]);
+        for (int i = step0; i < step1; i += WG_AHEAD) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 q = raws[0][j];
-            const int e = scale_exponent(scs[0][j]);
-            if (scs[0][j] == 0.f || (e != 255 && ((q.x | q.y | q.z | q.w) & 0x7f7f7f7fu) == 0u)) continue;
-            above = max(above, (e - top + WG_WINDOW - 1) / WG_WINDOW);
-            below = max(below, (top - e) / WG_WINDOW);
+          for (int a = 0; a < WG_AHEAD; ++a) fetch(i + a, raws[a], scs[a]);
+#pragma unroll
+          for (int a = 0; a < WG_AHEAD; ++a) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 q = raws[a][j];
+              const int e = scale_exponent(scs[a][j]);
+              if (scs[a][j] == 0.f || (e != 255 && ((q.x | q.y | q.z | q.w) & 0x7f7f7f7fu) == 0u)) continue;
+              above = max(above, (e - top + WG_WINDOW - 1) / WG_WINDOW);
+              below = max(below, (top - e) / WG_WINDOW);
+            }
           }
         }
         above = __reduce_max_sync(0xffffffffu, above);
